@@ -214,7 +214,9 @@ const char* infmoe_plugin_version(void); /* "1" */
  * device pointers unless named *_host; all launches are asynchronous on `hip_stream`. */
 
 enum { INFMOE_NORM_NONE = 0, INFMOE_NORM_RMS = 1, INFMOE_NORM_CENTERED = 2 };
-enum { INFMOE_FFN_RELU = 0, INFMOE_FFN_GATED_GELU = 1 };
+enum { INFMOE_FFN_RELU = 0, INFMOE_FFN_GATED_GELU = 1, INFMOE_FFN_GATED_SILU = 2 /* infmoe_experts_topk only */ };
+enum { INFMOE_DTYPE_F32 = 0, INFMOE_DTYPE_F16 = 1, INFMOE_DTYPE_BF16 = 2 };
+enum { INFMOE_SCORE_SOFTMAX = 0, INFMOE_SCORE_SIGMOID = 1 };
 
 /*
  * Fused gating: replaces layernorm_gpu + cublasSgemm_v2 + moe_expert_select
@@ -288,6 +290,28 @@ size_t infmoe_t5ff_weight_bytes(int32_t d, int32_t h, int32_t ffn_kind);
 size_t infmoe_t5ff_workspace_bytes(int32_t rows, int32_t d, int32_t h, int32_t ffn_kind);
 int32_t infmoe_t5ff_run(int32_t rows, int32_t d, int32_t h, int32_t norm_kind, int32_t ffn_kind, const void* weights,
                         const float* in, float* out, void* workspace, void* hip_stream);
+
+/* ---------------------------------------------------------------- several experts per token
+ * No counterpart in the reference, whose layer sends a token to one expert.  As above: device pointers, asynchronous on
+ * `hip_stream`, which belongs to the current device, as do the buffers; nothing is allocated, no host round trip, and a
+ * call may be captured into a graph after one eager call of its kind.  dtype: INFMOE_DTYPE_*; rows lie `stride` elements
+ * apart, their elements side by side. */
+
+/*
+ * Routing to the k best of E experts (1 <= E <= 1024, 1 <= k <= 32).  logits [T] rows of E in `dtype`.
+ *   s = softmax or logistic function of a row (score_kind);  c = s + bias (bias float [E] or NULL: of the choice only)
+ *   groups > 1 (a divisor of E, at most 64): of the E/groups experts of each group the group_top (1 or 2) largest c are
+ *     added, and the experts of the top_groups groups with the largest sums stay (k <= top_groups * E/groups)
+ *   ids[t][0..k) = the experts with the largest c, largest first, the lowest index among equals, groups likewise
+ *   weights[t][j] = scale * s of that expert, divided by the sum of the k chosen s when renormalize != 0
+ * Scores are compared as if computed in 64 bits; without a bias and with group_top == 1 the logits are compared (softmax
+ * and the logistic function keep their order).  An expert whose logit or bias is minus infinity is masked: it is not
+ * chosen, and where fewer than k are left the last slots get id -1 and weight 0.  A row that has no order (a NaN, an
+ * infinite logit under softmax, a bias of plus infinity) gets ids -1 and weights NaN.
+ */
+int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const void* logits, int64_t logits_stride,
+                          int32_t score_kind, const float* bias, int32_t groups, int32_t top_groups, int32_t group_top,
+                          int32_t renormalize, float scale, int32_t* ids, float* weights, void* hip_stream);
 
 #ifdef __cplusplus
 }

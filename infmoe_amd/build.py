@@ -35,6 +35,7 @@ SOURCES = [
     "kernels/gating.hip",
     "kernels/gating_slab.hip",
     "kernels/expert_skinny.hip",
+    "kernels/route.hip",
     "sublayers/t5ff_layer.cpp",
     "sublayers/sublayer.cpp",
     "npz_reader.cpp",

@@ -15,9 +15,11 @@ ERR_INVALID_ARGUMENT, ERR_UNKNOWN_FIELD, ERR_MISSING_FIELD, ERR_UNSUPPORTED = 1,
 ERR_IO, ERR_STATE, ERR_HIP, ERR_NAN = 5, 6, 7, 8
 FIELD_FLOAT32, FIELD_INT32, FIELD_CHAR, FIELD_UNKNOWN = 1, 5, 6, 8
 NORM_NONE, NORM_RMS, NORM_CENTERED = 0, 1, 2
-FFN_RELU, FFN_GATED_GELU = 0, 1
+FFN_RELU, FFN_GATED_GELU, FFN_GATED_SILU = 0, 1, 2
 NORM_KINDS = {"none": NORM_NONE, "rms": NORM_RMS, "centered": NORM_CENTERED}
 FFN_KINDS = {"relu": FFN_RELU, "gated_gelu": FFN_GATED_GELU}
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+SCORE_KINDS = {"softmax": 0, "sigmoid": 1}
 
 
 class Field(C.Structure):
@@ -32,6 +34,7 @@ class InfMoEError(RuntimeError):
 
 
 _vp, _i32, _sz = C.c_void_p, C.c_int32, C.c_size_t
+_i64, _f = C.c_int64, C.c_float
 _pi32, _pf = C.POINTER(C.c_int32), C.c_void_p  # device pointers travel as integers
 
 # name -> (restype, argtypes); every symbol include/infmoe.h declares
@@ -70,6 +73,7 @@ PROTOTYPES = {
     "infmoe_t5ff_weight_bytes": (_sz, [_i32, _i32, _i32]),
     "infmoe_t5ff_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "infmoe_t5ff_run": (_i32, [_i32, _i32, _i32, _i32, _i32, _vp, _pf, _pf, _vp, _vp]),
+    "infmoe_route_topk": (_i32, [_i32, _i32, _i32, _i32, _vp, _i64, _i32, _pf, _i32, _i32, _i32, _i32, _f, _vp, _pf, _vp]),
 }
 
 _lib = None

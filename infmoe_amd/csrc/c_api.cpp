@@ -373,4 +373,25 @@ int32_t infmoe_t5ff_run(int32_t rows, int32_t d, int32_t h, int32_t norm_kind, i
     });
 }
 
+// ---------------------------------------------------------------- several experts per token
+
+int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const void* logits, int64_t logits_stride,
+                          int32_t score_kind, const float* bias, int32_t groups, int32_t top_groups, int32_t group_top,
+                          int32_t renormalize, float scale, int32_t* ids, float* weights, void* hip_stream) {
+    return guarded([&]() -> int32_t {
+        INFMOE_NEED(T >= 0 && E > 0 && E <= kRouteMaxExperts, "route_topk: bad sizes (1 to 1024 experts)");
+        INFMOE_NEED(dtype >= DTYPE_F32 && dtype <= DTYPE_BF16, "route_topk: bad dtype");
+        INFMOE_NEED(score_kind == SCORE_SOFTMAX || score_kind == SCORE_SIGMOID, "route_topk: bad score_kind");
+        INFMOE_NEED(groups >= 1 && groups <= kRouteMaxGroups && E % groups == 0, "route_topk: groups must be 1 to 64 and divide the experts");
+        INFMOE_NEED(top_groups >= 1 && top_groups <= groups, "route_topk: top_groups must be 1 to groups");
+        INFMOE_NEED(group_top == 1 || (group_top == 2 && E / groups >= 2), "route_topk: group_top must be 1, or 2 with groups of two or more");
+        INFMOE_NEED(k >= 1 && k <= kRouteMaxTopK && k <= top_groups * (E / groups), "route_topk: k must be 1 to 32 and at most the experts that stay");
+        INFMOE_NEED(T <= 1 || logits_stride >= E, "route_topk: rows overlap");
+        INFMOE_NEED(T == 0 || (logits && ids && weights), "route_topk: null pointer");
+        INFMOE_HIP(launch_route_topk(T, E, k, logits, dtype, logits_stride, score_kind, bias, groups, top_groups, group_top,
+                                     renormalize != 0, scale, ids, weights, static_cast<hipStream_t>(hip_stream)));
+        return INFMOE_OK;
+    });
+}
+
 }  // extern "C"

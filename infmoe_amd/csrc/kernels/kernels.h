@@ -14,7 +14,9 @@
 namespace infmoe {
 
 enum NormKind : int32_t { NORM_NONE = 0, NORM_RMS = 1, NORM_CENTERED = 2 };
-enum FfnKind : int32_t { FFN_RELU = 0, FFN_GATED_GELU = 1 };
+enum FfnKind : int32_t { FFN_RELU = 0, FFN_GATED_GELU = 1, FFN_GATED_SILU = 2 };  // (the last one: launch_experts_topk only)
+enum DataType : int32_t { DTYPE_F32 = 0, DTYPE_F16 = 1, DTYPE_BF16 = 2 };
+enum ScoreKind : int32_t { SCORE_SOFTMAX = 0, SCORE_SIGMOID = 1 };
 
 constexpr float kNormEps = 1e-6f;  // plugin/MoELayerPlugin.cc:324, plugin/sublayers/T5FFLayer.cc:102
 
@@ -217,6 +219,14 @@ constexpr int kSkinnyMaxRows = 8;
 hipError_t launch_expert_skinny(const GemmProblem& p, int rows, hipStream_t stream);
 hipError_t launch_expert_skinny_grouped(const GemmProblem& p, size_t weight_stride, const int* count,
                                         const int* offset, int E, hipStream_t stream);
+
+// ---- routing to the k best experts (no counterpart in the reference, whose layer routes to one)
+// Limits: 1 <= E <= kRouteMaxExperts, 1 <= k <= min(kRouteMaxTopK, experts of top_groups groups), groups <= kRouteMaxGroups
+// and a divisor of E, group_top 1 or 2 (2 only with groups of two experts or more).
+constexpr int kRouteMaxExperts = 1024, kRouteMaxTopK = 32, kRouteMaxGroups = 64;
+hipError_t launch_route_topk(int T, int E, int k, const void* logits, int dtype, long long row_stride, int score,
+                             const float* bias, int groups, int top_groups, int group_top, bool renormalize, float scale,
+                             int* ids, float* weights, hipStream_t stream);
 
 // Kernels whose dynamic LDS exceeds 64 KB need the limit raised once per device.  Doing it on the
 // first launch only keeps later launches free of runtime calls other than the launch itself, so a

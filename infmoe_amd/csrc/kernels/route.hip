@@ -1,0 +1,329 @@
+// Routing to the k best experts for gfx950: scores, groups, selection and weights in one launch.
+//
+//   s_e = softmax(l)_e or 1 / (1 + exp(-l_e));  c_e = s_e + bias_e;  the `top_groups` groups with the largest sums of their
+//   `group_top` largest c stay;  ids = the k largest c, largest first, the lowest index among equals;
+//   w = scale * s_ids (/ sum of s_ids when renormalised).
+//
+// Softmax and the logistic function keep the order of the logits, so where neither a bias nor a sum over a group enters,
+// the logits themselves are compared, which needs no arithmetic and no tolerance.  Otherwise the choice is made on scores
+// in FP32, and a row in which two neighbours of the ranking are closer than what FP32 can order (see kScoreError) is
+// chosen once more on scores in 64 bits; a result never depends on FP32's roundings.
+//
+// Layout: a row of E logits takes 16, 32 or 64 neighbouring lanes of a wave, each with V <= 32 consecutive experts in
+// registers; a group of experts takes a power of two of those lanes (slots that this leaves over hold minus infinity).
+// Consecutive experts sit in ascending lanes and slots, so "the lowest index" is "the first lane, then the first slot",
+// and all exchanges are between registers of one wave: no LDS, no barrier.
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include "kernels.h"
+
+namespace infmoe {
+namespace {
+
+constexpr int kThreads = 256;
+typedef unsigned long long u64;
+constexpr float kInf = __builtin_inff();
+
+struct Args {
+    const void* logits;
+    long long stride;  // elements between rows
+    const float* bias;
+    int* ids;
+    float* weights;
+    int T, E, k, dtype, score, groups, per, lanes_log2, top_groups, group_top, renormalize, vec;
+    float scale;
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, false);
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, false), lo);
+}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+
+// Reductions over the G lanes of a row, the result in all of them.  Inside 16 lanes by data-parallel moves (lane ^ 1,
+// lane ^ 2, mirror in 8, mirror in 16), beyond by two exchanges through the LDS crossbar.
+template <int G, typename R>
+__device__ __forceinline__ R row_max(R v) {
+    v = larger(v, dpp<0xB1>(v));
+    v = larger(v, dpp<0x4E>(v));
+    v = larger(v, dpp<0x141>(v));
+    v = larger(v, dpp<0x140>(v));
+    if (G > 16) v = larger(v, __shfl_xor(v, 16));
+    if (G > 32) v = larger(v, __shfl_xor(v, 32));
+    return v;
+}
+template <int G, typename R>
+__device__ __forceinline__ R row_sum(R v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    if (G > 16) v += __shfl_xor(v, 16);
+    if (G > 32) v += __shfl_xor(v, 32);
+    return v;
+}
+
+__device__ __forceinline__ float load_logit(const Args& a, long long at) {
+    if (a.dtype == DTYPE_F32) return static_cast<const float*>(a.logits)[at];
+    const unsigned short h = static_cast<const unsigned short*>(a.logits)[at];
+    return a.dtype == DTYPE_BF16 ? __uint_as_float((unsigned)h << 16) : __half2float(__ushort_as_half(h));
+}
+
+__device__ __forceinline__ float exp_of(float x) { return __expf(x); }
+
+// Two scores p + bias computed in FP32 are ordered as the exact ones when they lie further apart than
+//   kScoreError * max(p_max, 2^-10) + 2^-22 * |p + bias|.
+// exp_of(x) is 2^(x * log2 e) with the product rounded, so its relative error is at most (1.45 |x| + 2) u, u = 2^-24; a
+// logistic score p = 1 / (1 + exp(-l)) turns that into p (1 - p) (1.45 |l| + 2) u + 2 u p <= 4 u, and where all scores are
+// small, p <= 2^-10, into less than 16 u * 2^-10.  A softmax score, p = exp(l - m) / sum, has the roundings of l - m and of
+// the argument, (2.45 |l - m| + 2) u p with |l - m| p <= 0.37 p_max, those of the sum, at most (log2 E + 2) u p, and the
+// quotient's, all in all under 16 u p_max.  The sum with the bias is rounded once: u |p + bias|.  Two such errors, either way.
+constexpr float kScoreError = 0x1p-19f;  // 32 u
+
+// The choice of the k best of one row per G lanes.  R: float, or double for the rows that FP32 cannot order.  Lane j of the
+// row gets the j-th expert in *mine (-1: nothing left to choose).  Returns whether the row is ordered for certain
+// (CHECK; the same answer in all of a row's lanes).
+template <typename R, bool CHECK, int G, int V>
+__device__ __forceinline__ bool choose(const Args& a, R (&c)[V], float floor_gap, int in_row, u64 row_lanes, int first, int* mine) {
+    const int lane = threadIdx.x & 63;
+    bool sure = true;
+    if (a.groups > 1) {
+        R one = -INFINITY, two = -INFINITY;  // the two largest of the lane's, then of its group's lanes
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            two = larger(two, one < c[i] ? one : c[i]);
+            one = larger(one, c[i]);
+        }
+        for (int step = 1; step < (1 << a.lanes_log2); step <<= 1) {
+            const R o1 = __shfl_xor(one, step), o2 = __shfl_xor(two, step);
+            two = larger(larger(two, o2), one < o1 ? one : o1);
+            one = larger(one, o1);
+        }
+        const R value = a.group_top == 2 ? one + two : one;
+        const int group = in_row >> a.lanes_log2;
+        int rank = 0;
+        for (int g = 0; g < a.groups; ++g) {
+            const R other = __shfl(value, (lane - in_row) + (g << a.lanes_log2));
+            rank += other > value || (other == value && g < group);
+            if (CHECK && g != group && group < a.groups && other > -INFINITY && value > -INFINITY)
+                sure = sure && fabs((double)(other - value)) > 2 * floor_gap + 0x1p-21 * fabs((double)value);
+        }
+        if (rank >= a.top_groups)
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = -INFINITY;
+    }
+    R before = INFINITY;
+    const int rounds = CHECK ? a.k + 1 : a.k;  // the border to the first expert left out counts too
+    for (int j = 0; j < rounds; ++j) {
+        R best = c[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = larger(best, c[i]);
+        const R top = row_max<G>(best);
+        if (CHECK && j > 0 && top > -INFINITY) sure = sure && (float)(before - top) > floor_gap + 0x1p-22f * fabsf((float)before);
+        if (j == a.k) break;
+        before = top;
+        const u64 who = __ballot(best == top) & row_lanes;
+        const int winner = (who != 0 ? __ffsll((long long)who) : 1) - 1;
+        int slot = 0;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) slot = c[i] == best ? i : slot;
+        const int expert = __shfl(first + slot, winner);
+        if (in_row == j) *mine = top > -INFINITY ? expert : -1;
+        if (lane == winner)
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = i == slot ? (R)-INFINITY : c[i];
+    }
+    return sure;
+}
+
+template <int G, int V>
+__global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
+    const int lane = threadIdx.x & 63, in_row = lane & (G - 1);
+    const u64 row_lanes = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1)) << (lane - in_row);
+    const long long row = ((long long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * (64 / G) + lane / G;
+    const bool live = row < a.T;
+    const long long at = (live ? row : a.T - 1) * a.stride;  // lanes past the last row repeat it and store nothing
+    const int group = in_row >> a.lanes_log2;
+    const int local = (in_row & ((1 << a.lanes_log2) - 1)) * V;  // of the lane's first expert in its group
+    const int first = group * a.per + local;
+    const int have = group < a.groups ? min(max(a.per - local, 0), V) : 0;
+
+    float l[V];
+    if (a.vec) {  // every slot taken, 16-byte pieces
+        if constexpr (V % 4 == 0) {
+            if (a.dtype == DTYPE_F32) {
+                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + at + first);
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i) {
+                    const float4 q = p[i];
+                    l[4 * i] = q.x, l[4 * i + 1] = q.y, l[4 * i + 2] = q.z, l[4 * i + 3] = q.w;
+                }
+            }
+        }
+        if constexpr (V % 8 == 0) {
+            if (a.dtype != DTYPE_F32) {
+                const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.logits) + at + first);
+#pragma unroll
+                for (int i = 0; i < V / 8; ++i) {
+                    const uint4 q = p[i];
+                    const unsigned u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (a.dtype == DTYPE_BF16) {
+                            l[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+                            l[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                        } else {
+                            l[8 * i + 2 * j] = __half2float(__ushort_as_half((unsigned short)(u[j] & 0xffff)));
+                            l[8 * i + 2 * j + 1] = __half2float(__ushort_as_half((unsigned short)(u[j] >> 16)));
+                        }
+                    }
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) l[i] = i < have ? load_logit(a, at + first + i) : -kInf;
+    }
+
+    bool bad = false;  // no order: a NaN, or a softmax over an infinite logit
+#pragma unroll
+    for (int i = 0; i < V; ++i) bad |= l[i] != l[i] || (a.score == SCORE_SOFTMAX && l[i] == kInf);
+
+    const bool scored = a.bias != nullptr || a.group_top == 2;
+    float m = 0.f, sum = 1.f;
+    if (a.score == SCORE_SOFTMAX) {
+        m = l[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) m = fmaxf(m, l[i]);
+        m = row_max<G>(m);
+        m = m > -kInf ? m : 0.f;  // (every expert masked)
+        if (scored || !a.renormalize) {
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum += exp_of(l[i] - m);
+            sum = row_sum<G>(sum);
+        }
+    }
+
+    int mine = -1;
+    if (!scored) {
+        float c[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = l[i];
+        choose<float, false, G, V>(a, c, 0.f, in_row, row_lanes, first, &mine);
+    } else {
+        float c[V], b[V], peak = 0x1p-10f;
+        const float rsum = 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            b[i] = a.bias != nullptr && i < have ? a.bias[first + i] : 0.f;
+            const float p = a.score == SCORE_SOFTMAX ? exp_of(l[i] - m) * rsum : 1.f / (1.f + exp_of(-l[i]));
+            peak = fmaxf(peak, p);
+            c[i] = l[i] > -kInf ? p + b[i] : -kInf;
+            bad |= !(c[i] < kInf);
+        }
+        peak = row_max<G>(peak);
+        bool sure = choose<float, true, G, V>(a, c, kScoreError * peak, in_row, row_lanes, first, &mine);
+        if (__ballot(!sure && !bad) != 0) {  // some row of this wave: all of its rows again, in 64 bits
+            double d[V], total = 0.0;
+            if (a.score == SCORE_SOFTMAX) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) total += exp((double)l[i] - m);
+                total = row_sum<G>(total);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double p = a.score == SCORE_SOFTMAX ? exp((double)l[i] - m) / total : 1.0 / (1.0 + exp(-(double)l[i]));
+                d[i] = l[i] > -kInf ? p + (double)b[i] : -INFINITY;
+            }
+            mine = -1;
+            choose<double, false, G, V>(a, d, 0.f, in_row, row_lanes, first, &mine);
+        }
+    }
+    const bool nan_row = (__ballot(bad) & row_lanes) != 0;
+
+    // Weights.  Renormalised ones are formed relative to the largest chosen logit, so that a row of tiny scores (their sum
+    // may be below FP32's range) keeps its ratios: softmax's common factor cancels; of the logistic function exp(l) / (1 + exp(l)).
+    const bool filled = in_row < a.k && mine >= 0;
+    const float x = filled ? load_logit(a, at + mine) : -kInf;
+    float w;
+    if (a.score == SCORE_SOFTMAX) {
+        const float base = a.renormalize ? row_max<G>(x) : m;
+        w = filled ? expf(x - base) : 0.f;
+        if (!a.renormalize && filled) w /= sum;
+    } else {
+        const float base = a.renormalize ? fminf(row_max<G>(x), 0.f) : 0.f;
+        w = !filled ? 0.f : x >= 0.f ? 1.f / (1.f + expf(-x)) : expf(x - base) / (1.f + expf(x));
+    }
+    if (a.renormalize) {
+        const float total = row_sum<G>(w);
+        w = total > 0.f ? w / total : w;
+    }
+    if (live && in_row < a.k) {
+        a.ids[row * a.k + in_row] = nan_row ? -1 : mine;
+        a.weights[row * a.k + in_row] = nan_row ? __builtin_nanf("") : a.scale * w;
+    }
+}
+
+template <int G, int V>
+hipError_t go(const Args& a, hipStream_t stream) {
+    const int rows = kThreads / G;
+    route_kernel<G, V><<<(a.T + rows - 1) / rows, kThreads, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+template <int G>
+hipError_t go_v(const Args& a, int v, hipStream_t stream) {
+    switch (v) {
+        case 1: return go<G, 1>(a, stream);
+        case 2: return go<G, 2>(a, stream);
+        case 4: return go<G, 4>(a, stream);
+        case 8: return go<G, 8>(a, stream);
+        case 16: return go<G, 16>(a, stream);
+        default: break;
+    }
+    if constexpr (G == 64) return go<64, 32>(a, stream);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_route_topk(int T, int E, int k, const void* logits, int dtype, long long row_stride, int score,
+                             const float* bias, int groups, int top_groups, int group_top, bool renormalize, float scale,
+                             int* ids, float* weights, hipStream_t stream) {
+    if (T <= 0) return hipSuccess;
+    Args a{logits, row_stride, bias, ids, weights, T, E, k, dtype, score, groups, E / groups, 0, top_groups, group_top, renormalize, 0, scale};
+    // As few lanes a row as hold it with at most 16 experts a lane (with 32 only where 64 lanes do not reach otherwise):
+    // a round of the selection costs a wave the same whether it serves one row or four, so rows side by side in one wave
+    // are the cheaper way through a batch.
+    int per_lane = 0, lanes = 16;
+    for (;; lanes *= 2) {
+        int parts = 1;
+        while (parts < groups) parts *= 2;  // groups, each of lanes / parts lanes
+        const bool fits = parts <= lanes && k <= lanes;
+        const int each = fits ? (a.per + lanes / parts - 1) / (lanes / parts) : 64;
+        if (each <= 16 || lanes == 64) {
+            if (each > 32) return hipErrorInvalidValue;  // (not reached: E <= 1024 and groups <= 64)
+            per_lane = 1;
+            while (per_lane < each) per_lane *= 2;
+            while ((parts << a.lanes_log2) < lanes) ++a.lanes_log2;
+            break;
+        }
+    }
+    const int size = dtype == DTYPE_F32 ? 4 : 2;
+    a.vec = a.per == (per_lane << a.lanes_log2) && (groups << a.lanes_log2) == lanes && per_lane * size % 16 == 0 &&
+            row_stride * size % 16 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
+    if (lanes == 16) return go_v<16>(a, per_lane, stream);
+    if (lanes == 32) return go_v<32>(a, per_lane, stream);
+    return go_v<64>(a, per_lane, stream);
+}
+
+}  // namespace infmoe
