@@ -313,6 +313,39 @@ int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const 
                           int32_t score_kind, const float* bias, int32_t groups, int32_t top_groups, int32_t group_top,
                           int32_t renormalize, float scale, int32_t* ids, float* weights, void* hip_stream);
 
+/*
+ * The experts' feed-forward products over such a routing:
+ *   y[t] = sum over j of weights[t][j] * wo_e act(wi_e x[t] [, wi_1_e x[t]]),  e = ids[t][j]
+ * ffn_kind: INFMOE_FFN_RELU max(u, 0); _GATED_GELU gelu_tanh(u) * v; _GATED_SILU u / (1 + exp(-u)) * v (wi_1 is NULL with
+ * RELU).  x, y [T] rows of d, wi, wi_1 [E] matrices [h][d] that lie wi_stride elements apart, wo [E] matrices [d][h]
+ * wo_stride apart (so the experts may be tensors of their own or slots of one packed block), all in `dtype`.  Sums are
+ * FP32; the hidden rows are rounded to `dtype` (they are the second product's operand), the weighted sum is FP32, in the
+ * order of j, and rounded once.  An id outside [0, E) adds 0 * weights[t][j]: nothing, or NaN where the weight is one.  Ids
+ * may repeat.  1 <= E <= 1024, 1 <= k <= 32, T * k <= 2^30.  d and h of whole 16-byte pieces and operands on 16-byte
+ * boundaries are the fast case, any others are served.  y must not overlap the inputs.
+ * workspace: infmoe_experts_topk_workspace_bytes, 256-byte aligned, of any contents, of one call at a time.
+ */
+size_t infmoe_experts_topk_workspace_bytes(int32_t T, int32_t k, int32_t E, int32_t d, int32_t h, int32_t dtype);
+int32_t infmoe_experts_topk(int32_t T, int32_t k, int32_t E, int32_t d, int32_t h, int32_t ffn_kind, int32_t dtype, const void* x,
+                            int64_t x_stride, const int32_t* ids, const float* weights, const void* wi, const void* wi_1,
+                            const void* wo, int64_t wi_stride, int64_t wo_stride, void* y, int64_t y_stride, void* workspace,
+                            void* hip_stream);
+
+/*
+ * A projection that all rows share, with a low-rank adapter per row (the requests of a batch bring their own):
+ *   y[t] = w x[t] + scale[a] * b_a (a_a x[t]),  a = adapter[t]
+ * w [n][d], a [L][r][d], b [L][n][r], x [T] rows of d, y [T] rows of n, all in `dtype`; adapter int32 [T], scale float [L]
+ * or NULL (1).  A row whose adapter is outside [0, L) gets w x[t].  Sums are FP32; scale[a] * a_a x[t] is rounded to
+ * `dtype` (it is the second product's operand), y once.  What one adapter holds cannot reach the rows of another.
+ * 1 <= r <= 256.  Rows of whole 16-byte pieces on 16-byte boundaries are the fast case.  Rows may come in any order; those
+ * of one adapter side by side are the cheap one.  y must not overlap the inputs.
+ * workspace: infmoe_lora_project_workspace_bytes, 256-byte aligned, of any contents, of one call at a time.
+ */
+size_t infmoe_lora_project_workspace_bytes(int32_t T, int32_t d, int32_t n, int32_t r, int32_t dtype);
+int32_t infmoe_lora_project(int32_t T, int32_t d, int32_t n, int32_t r, int32_t L, int32_t dtype, const void* x, int64_t x_stride,
+                            const void* w, const void* a, const void* b, const int32_t* adapter, const float* scale, void* y,
+                            int64_t y_stride, void* workspace, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,8 @@ SOURCES = [
     "kernels/gating_slab.hip",
     "kernels/expert_skinny.hip",
     "kernels/route.hip",
+    "kernels/experts_topk.hip",
+    "kernels/lora.hip",
     "sublayers/t5ff_layer.cpp",
     "sublayers/sublayer.cpp",
     "npz_reader.cpp",

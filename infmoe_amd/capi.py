@@ -20,6 +20,7 @@ NORM_KINDS = {"none": NORM_NONE, "rms": NORM_RMS, "centered": NORM_CENTERED}
 FFN_KINDS = {"relu": FFN_RELU, "gated_gelu": FFN_GATED_GELU}
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 SCORE_KINDS = {"softmax": 0, "sigmoid": 1}
+TOPK_FFN_KINDS = {**FFN_KINDS, "gated_silu": FFN_GATED_SILU}  # infmoe_experts_topk
 
 
 class Field(C.Structure):
@@ -74,6 +75,10 @@ PROTOTYPES = {
     "infmoe_t5ff_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "infmoe_t5ff_run": (_i32, [_i32, _i32, _i32, _i32, _i32, _vp, _pf, _pf, _vp, _vp]),
     "infmoe_route_topk": (_i32, [_i32, _i32, _i32, _i32, _vp, _i64, _i32, _pf, _i32, _i32, _i32, _i32, _f, _vp, _pf, _vp]),
+    "infmoe_experts_topk_workspace_bytes": (_sz, [_i32] * 6),
+    "infmoe_experts_topk": (_i32, [_i32] * 7 + [_vp, _i64, _vp, _pf, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "infmoe_lora_project_workspace_bytes": (_sz, [_i32] * 5),
+    "infmoe_lora_project": (_i32, [_i32] * 6 + [_vp, _i64, _vp, _vp, _vp, _vp, _pf, _vp, _i64, _vp, _vp]),
 }
 
 _lib = None

@@ -394,4 +394,52 @@ int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const 
     });
 }
 
+// (sizes that are refused below get zero)
+size_t infmoe_experts_topk_workspace_bytes(int32_t T, int32_t k, int32_t E, int32_t d, int32_t h, int32_t dtype) {
+    if (T <= 0 || k <= 0 || E <= 0 || d <= 0 || h <= 0) return 0;
+    return experts_topk_workspace_bytes(T, k, E, d, h, dtype);
+}
+
+int32_t infmoe_experts_topk(int32_t T, int32_t k, int32_t E, int32_t d, int32_t h, int32_t ffn_kind, int32_t dtype, const void* x,
+                            int64_t x_stride, const int32_t* ids, const float* weights, const void* wi, const void* wi_1,
+                            const void* wo, int64_t wi_stride, int64_t wo_stride, void* y, int64_t y_stride, void* workspace,
+                            void* hip_stream) {
+    return guarded([&]() -> int32_t {
+        INFMOE_NEED(T >= 0 && E > 0 && E <= kRouteMaxExperts && k > 0 && k <= kRouteMaxTopK, "experts_topk: bad sizes (1 to 1024 experts, 1 to 32 a token)");
+        INFMOE_NEED((int64_t)T * k <= (1 << 30), "experts_topk: too many rows");
+        INFMOE_NEED(d > 0 && h > 0 && d <= kRowsMaxLength && h <= kRowsMaxLength, "experts_topk: bad row length");
+        INFMOE_NEED(ffn_kind >= FFN_RELU && ffn_kind <= FFN_GATED_SILU, "experts_topk: bad ffn_kind");
+        INFMOE_NEED(dtype >= DTYPE_F32 && dtype <= DTYPE_BF16, "experts_topk: bad dtype");
+        INFMOE_NEED(T <= 1 || (x_stride >= d && y_stride >= d), "experts_topk: rows overlap");
+        INFMOE_NEED(E == 1 || (wi_stride >= (int64_t)h * d && wo_stride >= (int64_t)h * d), "experts_topk: experts overlap");
+        INFMOE_NEED(T == 0 || (x && ids && weights && wi && wo && y && workspace), "experts_topk: null pointer");
+        INFMOE_NEED(T == 0 || (wi_1 != nullptr) == (ffn_kind != FFN_RELU), "experts_topk: wi_1 goes with the gated kinds");
+        INFMOE_NEED((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "experts_topk: workspace must be 256-byte aligned");
+        INFMOE_HIP(launch_experts_topk(T, k, E, d, h, ffn_kind, dtype, x, x_stride, ids, weights, wi, wi_1, wo, wi_stride, wo_stride, y,
+                                       y_stride, workspace, static_cast<hipStream_t>(hip_stream)));
+        return INFMOE_OK;
+    });
+}
+
+size_t infmoe_lora_project_workspace_bytes(int32_t T, int32_t d, int32_t n, int32_t r, int32_t dtype) {
+    if (T <= 0 || d <= 0 || n <= 0 || r <= 0) return 0;
+    return lora_project_workspace_bytes(T, d, n, r, dtype);
+}
+
+int32_t infmoe_lora_project(int32_t T, int32_t d, int32_t n, int32_t r, int32_t L, int32_t dtype, const void* x, int64_t x_stride,
+                            const void* w, const void* a, const void* b, const int32_t* adapter, const float* scale, void* y,
+                            int64_t y_stride, void* workspace, void* hip_stream) {
+    return guarded([&]() -> int32_t {
+        INFMOE_NEED(T >= 0 && d > 0 && n > 0 && d <= kRowsMaxLength && n <= kRowsMaxLength, "lora_project: bad sizes");
+        INFMOE_NEED(r > 0 && r <= kLoraMaxRank && L > 0, "lora_project: bad adapters (rank 1 to 256)");
+        INFMOE_NEED(dtype >= DTYPE_F32 && dtype <= DTYPE_BF16, "lora_project: bad dtype");
+        INFMOE_NEED(T <= 1 || (x_stride >= d && y_stride >= n), "lora_project: rows overlap");
+        INFMOE_NEED(T == 0 || (x && w && a && b && adapter && y && workspace), "lora_project: null pointer");
+        INFMOE_NEED((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "lora_project: workspace must be 256-byte aligned");
+        INFMOE_HIP(launch_lora_project(T, d, n, r, L, dtype, x, x_stride, w, a, b, adapter, scale, y, y_stride, workspace,
+                                       static_cast<hipStream_t>(hip_stream)));
+        return INFMOE_OK;
+    });
+}
+
 }  // extern "C"

@@ -1,0 +1,291 @@
+// The experts' feed-forward products of a top-k routing for gfx950:
+//   y_t = sum_j weights[t][j] * wo_e act(wi_e x_t [, wi_1_e x_t]),  e = ids[t][j].
+//
+// Launches:
+//   plan     the slots (t, j) sorted by expert (stable: results do not depend on the order anything retires in) and cut
+//            into row tiles, on the device (calls of more than kPlanBlock slots count per block first);
+//   product  1: rows x_t gathered by slot, activation in the epilogue, hidden rows in the weights' type;
+//   product  2: hidden rows against wo, FP32 rows in slot order;
+//   combine  the k rows of a token, weighted and added in order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kernels.h"
+#include "row_gemm.h"
+
+namespace infmoe {
+namespace {
+
+using namespace rows;
+
+constexpr int kPlanBlock = 1024;  // slots ranked by one workgroup
+constexpr int kPlanWaves = kPlanBlock / 64;
+
+// ---------------------------------------------------------------- plan
+__global__ __launch_bounds__(kPlanBlock) void plan_count_kernel(int S, int E, const int* __restrict__ ids, int* __restrict__ hist) {
+    extern __shared__ int s_hist[];
+    for (int e = threadIdx.x; e < E; e += kPlanBlock) s_hist[e] = 0;
+    __syncthreads();
+    const int s = blockIdx.x * kPlanBlock + threadIdx.x;
+    const int e = s < S ? ids[s] : -1;
+    if (e >= 0 && e < E) atomicAdd(&s_hist[e], 1);  // integer sums: order-free
+    __syncthreads();
+    for (int i = threadIdx.x; i < E; i += kPlanBlock) hist[(size_t)blockIdx.x * E + i] = s_hist[i];
+}
+
+// Exclusive prefix of v over the workgroup's kPlanBlock threads; *total: the sum.
+__device__ __forceinline__ int block_prefix(int v, int* s_wave, int* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int run = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(run, d);
+        if (lane >= d) run += up;
+    }
+    if (lane == 63) s_wave[wave] = run;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        before += w < wave ? s_wave[w] : 0;
+        all += s_wave[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + run - v;
+}
+
+// row_slot[r]: slot of the r-th row in expert order; tiles / n_tiles: its cut into tiles of at most tile_rows rows.  Slots
+// whose id is no expert get no row.  Every workgroup adds up the blocks' counts itself, so that no launch lies between
+// counting and placing; one block (hist null) needs no counts of others.
+__global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(int S, int E, const int* __restrict__ ids, const int* __restrict__ hist,
+                                                                int tile_rows, int* __restrict__ row_slot, int4* __restrict__ tiles,
+                                                                int* __restrict__ n_tiles) {
+    extern __shared__ int s_dyn[];  // [kPlanWaves][E]: rows of each expert in this block, by wave
+    __shared__ int s_wave[kPlanWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanBlock) s_dyn[i] = 0;
+    __syncthreads();
+    const int s = blockIdx.x * kPlanBlock + threadIdx.x;
+    int e = s < S ? ids[s] : -1;
+    if (e >= E) e = -1;
+    const bool valid = e >= 0;
+    // lanes of this wave with the same expert: one ballot per bit of the index
+    unsigned long long same = __ballot(valid);
+    for (int bit = 0; (1 << bit) < E; ++bit) {
+        const unsigned long long m = __ballot(valid && ((e >> bit) & 1));
+        same &= (e >> bit) & 1 ? m : ~m;
+    }
+    const int rank = __popcll(same & (lane == 0 ? 0ull : ~0ull >> (64 - lane)));
+    if (valid && rank == 0) s_dyn[wave * E + e] = __popcll(same);
+    __syncthreads();
+    // thread i: expert i (E <= kPlanBlock)
+    const int i = threadIdx.x;
+    int count = 0, earlier = 0;
+    if (i < E) {
+        if (hist == nullptr) {
+            for (int w = 0; w < kPlanWaves; ++w) count += s_dyn[w * E + i];
+        } else {
+            for (int b = 0; b < (int)gridDim.x; ++b) {
+                const int c = hist[(size_t)b * E + i];
+                earlier += b < (int)blockIdx.x ? c : 0;
+                count += c;
+            }
+        }
+    }
+    int total = 0;
+    const int offset = block_prefix(count, s_wave, &total);
+    if (i < E) {
+        int run = offset + earlier;
+        for (int w = 0; w < kPlanWaves; ++w) {
+            const int c = s_dyn[w * E + i];
+            s_dyn[w * E + i] = run;
+            run += c;
+        }
+    }
+    if (blockIdx.x == 0) {
+        const int mine = (count + tile_rows - 1) / tile_rows;
+        int n = 0;
+        const int first = block_prefix(mine, s_wave, &n);
+        for (int j = 0; j < mine; ++j) tiles[first + j] = int4{i, offset + j * tile_rows, min(tile_rows, count - j * tile_rows), 0};
+        if (i == 0) *n_tiles = n;
+    }
+    __syncthreads();
+    if (valid) row_slot[s_dyn[wave * E + e] + rank] = s;
+}
+
+// ---------------------------------------------------------------- products
+struct Product {
+    const char* a;             // rows
+    const char *b, *b1;        // weights of expert 0 (b1: the second matrix of a gated first product)
+    void* c;
+    const int* row_slot;
+    const int4* tiles;
+    const int* n_tiles;
+    long long a_stride, b_expert;  // bytes
+    int k_slots;               // slots per token (first product: row r is token row_slot[r] / k_slots)
+    int N, K, ffn;
+};
+
+// FIRST: A gathered, activation, C rows in expert order in T.  Otherwise A in expert order, C rows in slot order in FP32.
+template <typename T, typename S, bool FIRST, bool GATED, bool ALIGNED>
+__global__ __launch_bounds__(S::kThreads) void product_kernel(Product p) {
+    extern __shared__ __align__(16) char lds[];
+    constexpr int NM = GATED ? 2 : 1, kOut = S::kCols / NM;  // columns of C per tile
+    const int cols = (p.N + kOut - 1) / kOut;
+    const int t = blockIdx.x / cols;
+    if (t >= *p.n_tiles) return;
+    const int n0 = (blockIdx.x % cols) * kOut;
+    const int4 tile = p.tiles[t];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WN, wn = wave % S::WN;
+    const int row_bytes = p.K * (int)sizeof(T);
+    const char* pa[S::kPiecesA];
+    const char* pb[S::kPiecesB];
+#pragma unroll
+    for (int i = 0; i < S::kPiecesA; ++i) {
+        const int r = tile.y + min((tid >> 3) + i * (S::kThreads / 8), tile.z - 1);  // (rows past the tile's repeat its last)
+        pa[i] = p.a + (FIRST ? (long long)(p.row_slot[r] / p.k_slots) : (long long)r) * p.a_stride;
+    }
+#pragma unroll
+    for (int i = 0; i < S::kPiecesB; ++i) {
+        // a wave's FN column blocks are half of the first matrix, half of the second when there are two
+        const int v = (tid >> 3) + i * (S::kThreads / 8), w = v / (16 * S::FN), q = v % (16 * S::FN);
+        const int m = q / (16 * S::FN / NM), n = n0 + w * (16 * S::FN / NM) + q % (16 * S::FN / NM);
+        pb[i] = (m ? p.b1 : p.b) + tile.x * p.b_expert + (long long)min(n, p.N - 1) * row_bytes;
+    }
+    v4f acc[S::FM][S::FN];
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    multiply<T, S, ALIGNED>(acc, lds, pa, pb, row_bytes);
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) {
+        const int r = (wm * S::FM + i) * 16 + (lane & 15);
+        if (r >= tile.z) continue;
+        const int row = tile.y + r;
+#pragma unroll
+        for (int j = 0; j < S::FN / NM; ++j) {
+            const int n = n0 + (wn * (S::FN / NM) + j) * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (n + q >= p.N) continue;
+                if constexpr (FIRST)
+                    static_cast<T*>(p.c)[(size_t)row * p.N + n + q] = (T)activate<T>(p.ffn, acc[i][j][q], GATED ? acc[i][j + S::FN / 2][q] : 0.f);
+                else
+                    static_cast<float*>(p.c)[(size_t)p.row_slot[row] * p.N + n + q] = acc[i][j][q];
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- combine
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(int d, int k, int E, const int* __restrict__ ids, const float* __restrict__ weights,
+                                                      const float* __restrict__ post, T* __restrict__ y, long long y_stride) {
+    const size_t t = blockIdx.x;
+    for (int n = threadIdx.x + blockIdx.y * 256; n < d; n += 256 * gridDim.y) {
+        float sum = 0.f;
+        for (int j = 0; j < k; ++j) {
+            const int e = ids[t * k + j];
+            const float v = e >= 0 && e < E ? post[(t * k + j) * d + n] : 0.f;
+            sum += weights[t * k + j] * v;
+        }
+        y[t * y_stride + n] = (T)sum;
+    }
+}
+
+// ---------------------------------------------------------------- host
+struct Carve {
+    int *row_slot, *n_tiles, *hist;
+    int4* tiles;
+    char* hidden;
+    float* post;
+    size_t total;
+};
+constexpr int kMinTile = 64;
+
+Carve carve(int T, int k, int E, int d, int h, int dtype, char* base) {
+    const size_t S = (size_t)T * k, size = dtype == DTYPE_F32 ? 4 : 2;
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        char* at = base ? base + off : nullptr;
+        off += (bytes + 255) & ~(size_t)255;
+        return at;
+    };
+    Carve c;
+    c.row_slot = reinterpret_cast<int*>(take(4 * S));
+    c.n_tiles = reinterpret_cast<int*>(take(4));
+    c.hist = reinterpret_cast<int*>(take(4 * ((S + kPlanBlock - 1) / kPlanBlock) * E));
+    c.tiles = reinterpret_cast<int4*>(take(sizeof(int4) * (S / kMinTile + std::min<size_t>(E, S))));
+    c.hidden = take(S * h * size);
+    c.post = reinterpret_cast<float*>(take(S * d * 4));
+    c.total = off;
+    return c;
+}
+
+template <typename T, typename S, bool FIRST, bool GATED>
+hipError_t go(const Product& p, int max_tiles, bool aligned, hipStream_t stream) {
+    const int out = S::kCols / (GATED ? 2 : 1);
+    const long long grid = (long long)max_tiles * ((p.N + out - 1) / out);
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    if (aligned) {
+        if (const hipError_t err = allow_lds_once<product_kernel<T, S, FIRST, GATED, true>>(S::kLds); err != hipSuccess) return err;
+        product_kernel<T, S, FIRST, GATED, true><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
+    } else {
+        if (const hipError_t err = allow_lds_once<product_kernel<T, S, FIRST, GATED, false>>(S::kLds); err != hipSuccess) return err;
+        product_kernel<T, S, FIRST, GATED, false><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long long x_stride, const int* ids, const float* weights,
+               const T* wi, const T* wi_1, const T* wo, long long wi_stride, long long wo_stride, T* y, long long y_stride,
+               const Carve& c, hipStream_t stream) {
+    using S = Shape<1, 4, 4, 2>;
+    const int slots = Tn * k, blocks = (slots + kPlanBlock - 1) / kPlanBlock;
+    if (blocks > 1) plan_count_kernel<<<blocks, kPlanBlock, 4 * E, stream>>>(slots, E, ids, c.hist);
+    const size_t lds = 4 * (size_t)kPlanWaves * E;
+    if (const hipError_t err = allow_lds_once<plan_place_kernel>(4 * kPlanWaves * kRouteMaxExperts); err != hipSuccess) return err;
+    plan_place_kernel<<<blocks, kPlanBlock, lds, stream>>>(slots, E, ids, blocks > 1 ? c.hist : nullptr, S::kRows, c.row_slot, c.tiles, c.n_tiles);
+    const int max_tiles = slots / S::kRows + std::min(E, slots);
+    auto on16 = [](const void* p, long long stride) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (long long)sizeof(T))) & 15) == 0; };
+    Product p{};
+    p.row_slot = c.row_slot, p.tiles = c.tiles, p.n_tiles = c.n_tiles, p.k_slots = k, p.ffn = ffn;
+    p.a = reinterpret_cast<const char*>(x), p.a_stride = x_stride * sizeof(T);
+    p.b = reinterpret_cast<const char*>(wi), p.b1 = reinterpret_cast<const char*>(wi_1), p.b_expert = wi_stride * sizeof(T);
+    p.c = c.hidden, p.N = h, p.K = d;
+    const bool in_ok = d * sizeof(T) % 16 == 0 && on16(x, x_stride) && on16(wi, wi_stride) && on16(wi_1, 0);
+    hipError_t err = ffn == FFN_RELU ? go<T, S, true, false>(p, max_tiles, in_ok, stream) : go<T, S, true, true>(p, max_tiles, in_ok, stream);
+    if (err != hipSuccess) return err;
+    p.a = c.hidden, p.a_stride = (long long)h * sizeof(T);
+    p.b = reinterpret_cast<const char*>(wo), p.b1 = nullptr, p.b_expert = wo_stride * sizeof(T);
+    p.c = c.post, p.N = d, p.K = h;
+    err = go<T, S, false, false>(p, max_tiles, h * sizeof(T) % 16 == 0 && on16(wo, wo_stride), stream);
+    if (err != hipSuccess) return err;
+    combine_kernel<T><<<dim3(Tn, (d + 1023) / 1024), 256, 0, stream>>>(d, k, E, ids, weights, c.post, y, y_stride);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t experts_topk_workspace_bytes(int T, int k, int E, int d, int h, int dtype) { return carve(T, k, E, d, h, dtype, nullptr).total; }
+
+hipError_t launch_experts_topk(int T, int k, int E, int d, int h, int ffn, int dtype, const void* x, long long x_stride, const int* ids,
+                               const float* weights, const void* wi, const void* wi_1, const void* wo, long long wi_stride,
+                               long long wo_stride, void* y, long long y_stride, void* workspace, hipStream_t stream) {
+    if (T <= 0) return hipSuccess;
+    const Carve c = carve(T, k, E, d, h, dtype, static_cast<char*>(workspace));
+    auto typed = [&](auto zero) {
+        using E_ = decltype(zero);
+        return run<E_>(T, k, E, d, h, ffn, static_cast<const E_*>(x), x_stride, ids, weights, static_cast<const E_*>(wi),
+                       static_cast<const E_*>(wi_1), static_cast<const E_*>(wo), wi_stride, wo_stride, static_cast<E_*>(y), y_stride, c, stream);
+    };
+    if (dtype == DTYPE_F32) return typed(float{});
+    if (dtype == DTYPE_F16) return typed(_Float16{});
+    return typed(__bf16{});
+}
+
+}  // namespace infmoe

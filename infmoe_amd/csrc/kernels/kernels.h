@@ -228,6 +228,22 @@ hipError_t launch_route_topk(int T, int E, int k, const void* logits, int dtype,
                              const float* bias, int groups, int top_groups, int group_top, bool renormalize, float scale,
                              int* ids, float* weights, hipStream_t stream);
 
+// ---- the experts' products of a top-k routing (no counterpart in the reference)
+// E <= kRouteMaxExperts, k <= kRouteMaxTopK, T * k <= 2^30; wi / wo of expert e are wi_stride / wo_stride elements after
+// those of expert e - 1.
+size_t experts_topk_workspace_bytes(int T, int k, int E, int d, int h, int dtype);
+hipError_t launch_experts_topk(int T, int k, int E, int d, int h, int ffn, int dtype, const void* x, long long x_stride, const int* ids,
+                               const float* weights, const void* wi, const void* wi_1, const void* wo, long long wi_stride,
+                               long long wo_stride, void* y, long long y_stride, void* workspace, hipStream_t stream);
+
+// ---- a projection with a low-rank adapter per row (no counterpart in the reference)
+// w [n][d], a [L][r][d], b [L][n][r], r <= kLoraMaxRank; a row whose adapter is outside [0, L) has none; scale null: 1.
+constexpr int kLoraMaxRank = 256, kRowsMaxLength = 1 << 24;  // (a row's bytes fit 31 bits)
+size_t lora_project_workspace_bytes(int T, int d, int n, int r, int dtype);
+hipError_t launch_lora_project(int T, int d, int n, int r, int L, int dtype, const void* x, long long x_stride, const void* w, const void* a,
+                               const void* b, const int* adapter, const float* scale, void* y, long long y_stride, void* workspace,
+                               hipStream_t stream);
+
 // Kernels whose dynamic LDS exceeds 64 KB need the limit raised once per device.  Doing it on the
 // first launch only keeps later launches free of runtime calls other than the launch itself, so a
 // caller may capture them in a graph after one eager call.

@@ -1,0 +1,163 @@
+// A projection shared by all rows of a batch with a low-rank adapter per row, for gfx950:
+//   y_t = W x_t + scale_a * B_a (A_a x_t),  a = adapter[t].
+//
+// Two launches: `shrink` forms u_t = scale_a * A_a x_t ([T][r], in the operands' type, as the second product takes it);
+// `project` computes W x_t and, before its tile leaves the registers, goes over the adapters that occur among the tile's
+// rows and adds u_t B_a^T to the rows that use each: y is written once and never read.
+#include <hip/hip_runtime.h>
+
+#include "kernels.h"
+#include "row_gemm.h"
+
+namespace infmoe {
+namespace {
+
+using namespace rows;
+
+struct Args {
+    const char *x, *w, *a, *b;
+    char *u, *y;
+    const int* adapter;
+    const float* scale;
+    long long x_stride, y_stride;  // bytes
+    int T, d, n, r, L, u_stride;   // u_stride: bytes, a multiple of 16
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+    return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void shrink_kernel(Args p) {
+    const int t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int a = p.adapter[t];
+    if (a < 0 || a >= p.L) return;  // (its u is never used)
+    const T* x = reinterpret_cast<const T*>(p.x + t * p.x_stride);
+    const T* m = reinterpret_cast<const T*>(p.a) + (size_t)a * p.r * p.d;
+    const float s = p.scale != nullptr ? p.scale[a] : 1.f;
+    T* u = reinterpret_cast<T*>(p.u + (size_t)t * p.u_stride);
+    for (int j = wave; j < p.u_stride / (int)sizeof(T); j += 4) {
+        float sum = 0.f;
+        if (j < p.r)
+            for (int k = lane; k < p.d; k += 64) sum += (float)x[k] * (float)m[(size_t)j * p.d + k];
+        sum = wave_sum(sum);
+        if (lane == 0) u[j] = (T)(s * sum);
+    }
+}
+
+template <typename T, typename S, bool ALIGNED, bool B_ALIGNED>
+__global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ int s_adapter[S::kRows], s_list[S::kRows], s_n;
+    const int cols = (p.n + S::kCols - 1) / S::kCols;
+    const int row0 = blockIdx.x / cols * S::kRows, n0 = blockIdx.x % cols * S::kCols;
+    const int count = min(S::kRows, p.T - row0);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WN, wn = wave % S::WN;
+    const char* pa[S::kPiecesA];
+    const char* pb[S::kPiecesB];
+#pragma unroll
+    for (int i = 0; i < S::kPiecesA; ++i) pa[i] = p.x + (row0 + min((tid >> 3) + i * (S::kThreads / 8), count - 1)) * p.x_stride;
+    const int row_bytes = p.d * (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < S::kPiecesB; ++i) pb[i] = p.w + (long long)min(n0 + (tid >> 3) + i * (S::kThreads / 8), p.n - 1) * row_bytes;
+
+    // the adapters that occur in the tile, in the order of their first rows
+    for (int i = tid; i < S::kRows; i += S::kThreads) {
+        const int a = i < count ? p.adapter[row0 + i] : -1;
+        s_adapter[i] = a >= 0 && a < p.L ? a : -1;
+    }
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    if (tid < 64) {
+        int n = 0;
+        for (int i0 = 0; i0 < S::kRows; i0 += 64) {
+            const int i = i0 + lane, a = s_adapter[i];
+            bool first = a >= 0 && (i == 0 || s_adapter[i - 1] != a);  // (rows of a request lie side by side: seldom more work)
+            for (int j = 0; first && j < i - 1; ++j) first = s_adapter[j] != a;
+            const unsigned long long m = __ballot(first);
+            if (first) s_list[n + __popcll(m & (lane == 0 ? 0ull : ~0ull >> (64 - lane)))] = a;
+            n += __popcll(m);
+        }
+        if (lane == 0) s_n = n;
+    }
+    v4f acc[S::FM][S::FN];
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    multiply<T, S, ALIGNED>(acc, lds, pa, pb, row_bytes);  // (starts with a barrier)
+
+    int mine[S::FM];
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) mine[i] = s_adapter[(wm * S::FM + i) * 16 + (lane & 15)];
+#pragma unroll
+    for (int i = 0; i < S::kPiecesA; ++i) pa[i] = p.u + (size_t)(row0 + min((tid >> 3) + i * (S::kThreads / 8), count - 1)) * p.u_stride;
+    const int r_bytes = p.r * (int)sizeof(T);
+    for (int q = 0; q < s_n; ++q) {
+        const int a = s_list[q];
+        bool keep[S::FM];
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) keep[i] = mine[i] == a;
+#pragma unroll
+        for (int i = 0; i < S::kPiecesB; ++i)
+            pb[i] = p.b + ((long long)a * p.n + min(n0 + (tid >> 3) + i * (S::kThreads / 8), p.n - 1)) * r_bytes;
+        multiply_kept<T, S, B_ALIGNED>(acc, lds, pa, pb, r_bytes, keep);
+    }
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) {
+        const int r = (wm * S::FM + i) * 16 + (lane & 15);
+        if (r >= count) continue;
+        T* y = reinterpret_cast<T*>(p.y + (row0 + r) * p.y_stride);
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < p.n) y[n + q] = (T)acc[i][j][q];
+        }
+    }
+}
+
+template <typename T, typename S, bool ALIGNED, bool B_ALIGNED>
+hipError_t go(const Args& p, hipStream_t stream) {
+    const long long grid = (long long)((p.T + S::kRows - 1) / S::kRows) * ((p.n + S::kCols - 1) / S::kCols);
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    if (const hipError_t err = allow_lds_once<project_kernel<T, S, ALIGNED, B_ALIGNED>>(S::kLds); err != hipSuccess) return err;
+    project_kernel<T, S, ALIGNED, B_ALIGNED><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run(const Args& p, hipStream_t stream) {
+    using S = Shape<1, 4, 4, 2>;
+    shrink_kernel<T><<<p.T, 256, 0, stream>>>(p);
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | p.x_stride | p.d * sizeof(T)) & 15) == 0;
+    const bool b_aligned = ((reinterpret_cast<uintptr_t>(p.b) | p.r * sizeof(T)) & 15) == 0;
+    if (aligned) return b_aligned ? go<T, S, true, true>(p, stream) : go<T, S, true, false>(p, stream);
+    return b_aligned ? go<T, S, false, true>(p, stream) : go<T, S, false, false>(p, stream);
+}
+
+inline int u_stride_bytes(int r, int size) { return (r * size + 15) / 16 * 16; }
+
+}  // namespace
+
+size_t lora_project_workspace_bytes(int T, int, int, int r, int dtype) {
+    return ((size_t)T * u_stride_bytes(r, dtype == DTYPE_F32 ? 4 : 2) + 255) & ~(size_t)255;
+}
+
+hipError_t launch_lora_project(int T, int d, int n, int r, int L, int dtype, const void* x, long long x_stride, const void* w, const void* a,
+                               const void* b, const int* adapter, const float* scale, void* y, long long y_stride, void* workspace,
+                               hipStream_t stream) {
+    if (T <= 0) return hipSuccess;
+    const int size = dtype == DTYPE_F32 ? 4 : 2;
+    auto in = [](const void* p) { return static_cast<const char*>(p); };
+    const Args p{in(x), in(w), in(a), in(b), static_cast<char*>(workspace), static_cast<char*>(y), adapter, scale, x_stride * size, y_stride * size,
+                 T, d, n, r, L, u_stride_bytes(r, size)};
+    if (dtype == DTYPE_F32) return run<float>(p, stream);
+    if (dtype == DTYPE_F16) return run<_Float16>(p, stream);
+    return run<__bf16>(p, stream);
+}
+
+}  // namespace infmoe
