@@ -13,6 +13,7 @@
 
 #include "kernels.h"
 #include "row_gemm.h"
+#include "row_stream.h"
 
 namespace infmoe {
 namespace {
@@ -180,6 +181,87 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Product p) {
     }
 }
 
+// ---- few rows per expert: the weights streamed through the registers (row_stream.h)
+// Hidden rows in slot order here, so that calls of up to kMiniSlots slots need no plan: every wave finds the slots of its
+// expert among the ids by ballots.  (Up to 64 slots are one ballot; the t-th expert in use is that of the t-th slot whose
+// expert does not occur before it.)
+constexpr int kMiniSlots = 64;
+
+struct FewRows {
+    const int* ids;
+    int S, E;  // ids: null when there is a plan
+};
+
+template <typename T, int FM, int FN, bool FIRST, bool GATED, bool ALIGNED>
+__global__ __launch_bounds__(kStreamThreads) void stream_kernel(Product p, FewRows few) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ int s_slot[kMiniSlots];
+    constexpr int NM = GATED ? 2 : 1, kOut = 16 * FN / NM, kTile = 16 * FM;
+    const int cols = (p.N + kOut - 1) / kOut;
+    const int t = blockIdx.x / cols, n0 = blockIdx.x % cols * kOut;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int expert, count, first_row = 0;
+    if (few.ids != nullptr) {
+        int e = lane < few.S ? few.ids[lane] : -1;
+        const bool valid = e >= 0 && e < few.E;
+        unsigned long long same = __ballot(valid);
+        for (int bit = 0; (1 << bit) < few.E; ++bit) {
+            const unsigned long long m = __ballot(valid && ((e >> bit) & 1));
+            same &= (e >> bit) & 1 ? m : ~m;
+        }
+        const unsigned long long below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+        const bool first = valid && (same & below) == 0;
+        const unsigned long long firsts = __ballot(first);
+        const unsigned long long chosen = __ballot(first && __popcll(firsts & below) == t);
+        if (chosen == 0) return;  // fewer experts in use
+        expert = __builtin_amdgcn_readlane(e, __ffsll((long long)chosen) - 1);
+        const unsigned long long mine = __ballot(valid && e == expert);
+        count = __popcll(mine);
+        if (wave == 0 && valid && e == expert) s_slot[__popcll(mine & below)] = lane;
+        __syncthreads();
+    } else {
+        if (t >= *p.n_tiles) return;
+        const int4 tile = p.tiles[t];
+        expert = tile.x, first_row = tile.y, count = tile.z;
+    }
+    auto slot_of = [&](int r) { return few.ids != nullptr ? s_slot[r] : p.row_slot[first_row + r]; };
+    const int row_bytes = p.K * (int)sizeof(T), steps = (row_bytes + kStepBytes - 1) / kStepBytes;
+    const char* pw[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + j % (FN / NM) * 16 + (lane & 15);
+        pw[j] = (j >= FN / NM ? p.b1 : p.b) + expert * p.b_expert + (long long)min(n, p.N - 1) * row_bytes;
+    }
+    for (int r0 = 0; r0 < count; r0 += kTile) {  // (more than one round only without a plan)
+        const char* px[FM];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int slot = slot_of(min(r0 + i * 16 + (lane & 15), count - 1));
+            px[i] = p.a + (long long)(FIRST ? slot / p.k_slots : slot) * p.a_stride;
+        }
+        v4f acc[FM][FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, row_bytes);
+        if (r0 > 0) __syncthreads();  // the last round's sums have been taken
+        join_waves<FM, FN, NM>(lds, acc, [&](int i, int j, const v4f(&sum)[NM]) {
+            const int r = r0 + i * 16 + (lane & 15), n = n0 + j * 16 + (lane >> 4) * 4;
+            if (r >= count) return;
+            const size_t at = (size_t)slot_of(r) * p.N + n;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (n + q >= p.N) continue;
+                if constexpr (FIRST)
+                    static_cast<T*>(p.c)[at + q] = (T)activate<T>(p.ffn, sum[0][q], GATED ? sum[NM - 1][q] : 0.f);
+                else
+                    static_cast<float*>(p.c)[at + q] = sum[0][q];
+            }
+        });
+    }
+}
+
 // ---------------------------------------------------------------- combine
 template <typename T>
 __global__ __launch_bounds__(256) void combine_kernel(int d, int k, int E, const int* __restrict__ ids, const float* __restrict__ weights,
@@ -204,7 +286,7 @@ struct Carve {
     float* post;
     size_t total;
 };
-constexpr int kMinTile = 64;
+constexpr int kMinTile = 16;
 
 Carve carve(int T, int k, int E, int d, int h, int dtype, char* base) {
     const size_t S = (size_t)T * k, size = dtype == DTYPE_F32 ? 4 : 2;
@@ -240,30 +322,74 @@ hipError_t go(const Product& p, int max_tiles, bool aligned, hipStream_t stream)
     return hipGetLastError();
 }
 
+template <typename T, int FM, int FN, bool FIRST, bool GATED>
+hipError_t go_stream(const Product& p, const FewRows& few, int max_tiles, bool aligned, hipStream_t stream) {
+    constexpr int out = 16 * FN / (GATED ? 2 : 1), lds = stream_lds<FM, FN>();
+    const long long grid = (long long)max_tiles * ((p.N + out - 1) / out);
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    if (aligned) {
+        if (const hipError_t err = allow_lds_once<stream_kernel<T, FM, FN, FIRST, GATED, true>>(lds); err != hipSuccess) return err;
+        stream_kernel<T, FM, FN, FIRST, GATED, true><<<(int)grid, kStreamThreads, lds, stream>>>(p, few);
+    } else {
+        if (const hipError_t err = allow_lds_once<stream_kernel<T, FM, FN, FIRST, GATED, false>>(lds); err != hipSuccess) return err;
+        stream_kernel<T, FM, FN, FIRST, GATED, false><<<(int)grid, kStreamThreads, lds, stream>>>(p, few);
+    }
+    return hipGetLastError();
+}
+
+// Weight rows per workgroup: 64 (32 hidden columns of a gated product) where that leaves every compute unit two workgroups,
+// down to 16 otherwise.
+template <typename T, int FM, bool FIRST, bool GATED>
+hipError_t go_few(const Product& p, const FewRows& few, int max_tiles, bool aligned, hipStream_t stream) {
+    const long long blocks16 = (long long)max_tiles * ((p.N + 15) / 16) * (GATED ? 2 : 1);
+    if (blocks16 >= 4 * 512) return go_stream<T, FM, 4, FIRST, GATED>(p, few, max_tiles, aligned, stream);
+    if (GATED || blocks16 >= 2 * 512) return go_stream<T, FM, 2, FIRST, GATED>(p, few, max_tiles, aligned, stream);
+    if constexpr (!GATED) return go_stream<T, FM, 1, FIRST, GATED>(p, few, max_tiles, aligned, stream);
+    return hipErrorInvalidValue;
+}
+
 template <typename T>
 hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long long x_stride, const int* ids, const float* weights,
                const T* wi, const T* wi_1, const T* wo, long long wi_stride, long long wo_stride, T* y, long long y_stride,
                const Carve& c, hipStream_t stream) {
     using S = Shape<1, 4, 4, 2>;
     const int slots = Tn * k, blocks = (slots + kPlanBlock - 1) / kPlanBlock;
-    if (blocks > 1) plan_count_kernel<<<blocks, kPlanBlock, 4 * E, stream>>>(slots, E, ids, c.hist);
-    const size_t lds = 4 * (size_t)kPlanWaves * E;
-    if (const hipError_t err = allow_lds_once<plan_place_kernel>(4 * kPlanWaves * kRouteMaxExperts); err != hipSuccess) return err;
-    plan_place_kernel<<<blocks, kPlanBlock, lds, stream>>>(slots, E, ids, blocks > 1 ? c.hist : nullptr, S::kRows, c.row_slot, c.tiles, c.n_tiles);
-    const int max_tiles = slots / S::kRows + std::min(E, slots);
+    // few rows per expert: tiles of 16 or 32 rows, weights streamed
+    const int few_blocks = slots <= 4 * E ? 1 : slots <= 16 * E ? 2 : 0;
+    const bool mini = few_blocks > 0 && slots <= kMiniSlots;
+    const int tile_rows = few_blocks > 0 ? 16 * few_blocks : S::kRows;
+    if (!mini) {
+        if (blocks > 1) plan_count_kernel<<<blocks, kPlanBlock, 4 * E, stream>>>(slots, E, ids, c.hist);
+        const size_t lds = 4 * (size_t)kPlanWaves * E;
+        if (const hipError_t err = allow_lds_once<plan_place_kernel>(4 * kPlanWaves * kRouteMaxExperts); err != hipSuccess) return err;
+        plan_place_kernel<<<blocks, kPlanBlock, lds, stream>>>(slots, E, ids, blocks > 1 ? c.hist : nullptr, tile_rows, c.row_slot, c.tiles, c.n_tiles);
+    }
+    const int max_tiles = (mini ? 0 : slots / tile_rows) + std::min(E, slots);
     auto on16 = [](const void* p, long long stride) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (long long)sizeof(T))) & 15) == 0; };
+    const FewRows few{mini ? ids : nullptr, slots, E};
     Product p{};
     p.row_slot = c.row_slot, p.tiles = c.tiles, p.n_tiles = c.n_tiles, p.k_slots = k, p.ffn = ffn;
     p.a = reinterpret_cast<const char*>(x), p.a_stride = x_stride * sizeof(T);
     p.b = reinterpret_cast<const char*>(wi), p.b1 = reinterpret_cast<const char*>(wi_1), p.b_expert = wi_stride * sizeof(T);
     p.c = c.hidden, p.N = h, p.K = d;
     const bool in_ok = d * sizeof(T) % 16 == 0 && on16(x, x_stride) && on16(wi, wi_stride) && on16(wi_1, 0);
-    hipError_t err = ffn == FFN_RELU ? go<T, S, true, false>(p, max_tiles, in_ok, stream) : go<T, S, true, true>(p, max_tiles, in_ok, stream);
+    hipError_t err;
+    if (ffn == FFN_RELU)
+        err = few_blocks == 1   ? go_few<T, 1, true, false>(p, few, max_tiles, in_ok, stream)
+              : few_blocks == 2 ? go_few<T, 2, true, false>(p, few, max_tiles, in_ok, stream)
+                                : go<T, S, true, false>(p, max_tiles, in_ok, stream);
+    else
+        err = few_blocks == 1   ? go_few<T, 1, true, true>(p, few, max_tiles, in_ok, stream)
+              : few_blocks == 2 ? go_few<T, 2, true, true>(p, few, max_tiles, in_ok, stream)
+                                : go<T, S, true, true>(p, max_tiles, in_ok, stream);
     if (err != hipSuccess) return err;
     p.a = c.hidden, p.a_stride = (long long)h * sizeof(T);
     p.b = reinterpret_cast<const char*>(wo), p.b1 = nullptr, p.b_expert = wo_stride * sizeof(T);
     p.c = c.post, p.N = d, p.K = h;
-    err = go<T, S, false, false>(p, max_tiles, h * sizeof(T) % 16 == 0 && on16(wo, wo_stride), stream);
+    const bool out_ok = h * sizeof(T) % 16 == 0 && on16(wo, wo_stride);
+    err = few_blocks == 1   ? go_few<T, 1, false, false>(p, few, max_tiles, out_ok, stream)
+          : few_blocks == 2 ? go_few<T, 2, false, false>(p, few, max_tiles, out_ok, stream)
+                            : go<T, S, false, false>(p, max_tiles, out_ok, stream);
     if (err != hipSuccess) return err;
     combine_kernel<T><<<dim3(Tn, (d + 1023) / 1024), 256, 0, stream>>>(d, k, E, ids, weights, c.post, y, y_stride);
     return hipGetLastError();

@@ -8,11 +8,14 @@
 
 #include "kernels.h"
 #include "row_gemm.h"
+#include "row_stream.h"
 
 namespace infmoe {
 namespace {
 
 using namespace rows;
+
+constexpr int kFewShrink = 256;  // rows up to which u takes a wave per row and rank
 
 struct Args {
     const char *x, *w, *a, *b;
@@ -30,20 +33,82 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void shrink_kernel(Args p) {
-    const int t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ float dot_piece(v4u a, v4u b, float sum) {
+    union {
+        v4u v;
+        T e[16 / sizeof(T)];
+    } p{a}, q{b};
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); ++i) sum = fmaf((float)p.e[i], (float)q.e[i], sum);
+    return sum;
+}
+
+// u of few rows: a wave per row and rank.
+template <typename T, bool ALIGNED>
+__global__ __launch_bounds__(256) void shrink_few_kernel(Args p) {
+    const int t = blockIdx.x, lane = threadIdx.x & 63, j = blockIdx.y * 4 + (threadIdx.x >> 6);
     const int a = p.adapter[t];
-    if (a < 0 || a >= p.L) return;  // (its u is never used)
-    const T* x = reinterpret_cast<const T*>(p.x + t * p.x_stride);
-    const T* m = reinterpret_cast<const T*>(p.a) + (size_t)a * p.r * p.d;
-    const float s = p.scale != nullptr ? p.scale[a] : 1.f;
-    T* u = reinterpret_cast<T*>(p.u + (size_t)t * p.u_stride);
-    for (int j = wave; j < p.u_stride / (int)sizeof(T); j += 4) {
-        float sum = 0.f;
-        if (j < p.r)
-            for (int k = lane; k < p.d; k += 64) sum += (float)x[k] * (float)m[(size_t)j * p.d + k];
-        sum = wave_sum(sum);
-        if (lane == 0) u[j] = (T)(s * sum);
+    if (a < 0 || a >= p.L || j >= p.u_stride / (int)sizeof(T)) return;  // (a row without an adapter: its u is never used)
+    float sum = 0.f;
+    if (j < p.r) {
+        const int end = p.d * (int)sizeof(T);
+        const char *x = p.x + t * p.x_stride, *m = p.a + ((long long)a * p.r + j) * end;
+        int k = lane * 16;
+        for (; k + 3 * 1024 + 16 <= end; k += 4 * 1024) {
+            v4u q[4], w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = whole_piece<T, ALIGNED>(x + k + i * 1024), w[i] = whole_piece<T, ALIGNED>(m + k + i * 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = dot_piece<T>(q[i], w[i], sum);
+        }
+        for (; k < end; k += 1024) sum = dot_piece<T>(piece<T, ALIGNED>(x, k, end), piece<T, ALIGNED>(m, k, end), sum);
+        sum = wave_sum(sum) * (p.scale != nullptr ? p.scale[a] : 1.f);
+    }
+    if (lane == 0) reinterpret_cast<T*>(p.u + (size_t)t * p.u_stride)[j] = (T)sum;
+}
+
+// u of many rows: 16 * FM rows of a workgroup against the adapters that occur among them, 32 ranks at a time, on the matrix
+// cores (row_stream.h: A_a takes the place of the weights).
+template <typename T, int FM, bool ALIGNED>
+__global__ __launch_bounds__(kStreamThreads) void shrink_kernel(Args p) {
+    extern __shared__ __align__(16) char lds[];
+    constexpr int FN = 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row0 = blockIdx.x * 16 * FM, count = min(16 * FM, p.T - row0), j0 = blockIdx.y * 32;
+    const int end = p.d * (int)sizeof(T), steps = (end + kStepBytes - 1) / kStepBytes;
+    const int a_lane = lane < count ? p.adapter[row0 + lane] : -1;  // (16 * FM <= 64)
+    const char* px[FM];
+    int mine[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        px[i] = p.x + (row0 + min(i * 16 + (lane & 15), count - 1)) * p.x_stride;
+        mine[i] = __shfl(a_lane, i * 16 + (lane & 15));
+    }
+    unsigned long long left = __ballot(a_lane >= 0 && a_lane < p.L);
+    bool again = false;
+    while (left != 0) {  // (the same in all waves)
+        const int a = __builtin_amdgcn_readlane(a_lane, __ffsll((long long)left) - 1);
+        left &= ~__ballot(a_lane == a);
+        const char* pw[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) pw[j] = p.a + ((long long)a * p.r + min(j0 + j * 16 + (lane & 15), p.r - 1)) * end;
+        v4f acc[FM][FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, end);
+        if (again) __syncthreads();
+        again = true;
+        const float s = p.scale != nullptr ? p.scale[a] : 1.f;
+        join_waves<FM, FN, 1>(lds, acc, [&](int i, int j, const v4f(&sum)[1]) {
+            if (mine[i] != a) return;
+            T* u = reinterpret_cast<T*>(p.u + (size_t)(row0 + i * 16 + (lane & 15)) * p.u_stride);
+            const int n = j0 + j * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < p.u_stride / (int)sizeof(T)) u[n + q] = (T)(n + q < p.r ? s * sum[0][q] : 0.f);
+        });
     }
 }
 
@@ -120,6 +185,57 @@ __global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
     }
 }
 
+// Few rows: W streamed once through the registers, 16 * FN of its rows per workgroup; the adapters' part of an output is added
+// by the lane that holds the joined sum.
+template <typename T, int FM, int FN, bool ALIGNED, bool B_ALIGNED>
+__global__ __launch_bounds__(kStreamThreads) void project_few_kernel(Args p) {
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16 * FN, row0 = blockIdx.y * 16 * FM, count = min(16 * FM, p.T - row0);
+    const int end = p.d * (int)sizeof(T), steps = (end + kStepBytes - 1) / kStepBytes, r_end = p.r * (int)sizeof(T);
+    const char *px[FM], *pw[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) px[i] = p.x + (row0 + min(i * 16 + (lane & 15), count - 1)) * p.x_stride;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) pw[j] = p.w + (long long)min(n0 + j * 16 + (lane & 15), p.n - 1) * end;
+    v4f acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, end);
+    join_waves<FM, FN, 1>(lds, acc, [&](int i, int j, v4f(&sum)[1]) {
+        const int t = row0 + i * 16 + (lane & 15), n = n0 + j * 16 + (lane >> 4) * 4;
+        if (t >= p.T) return;
+        const int a = p.adapter[t];
+        if (a >= 0 && a < p.L) {
+            const char *u = p.u + (size_t)t * p.u_stride, *b = p.b + ((long long)a * p.n + n) * r_end;
+            for (int k = 0; k < r_end; k += 16) {
+                const v4u uk = *reinterpret_cast<const v4u*>(u + k);  // (u is padded to whole pieces)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (n + q < p.n) sum[0][q] = dot_piece<T>(uk, piece<T, B_ALIGNED>(b + q * r_end, k, r_end), sum[0][q]);
+            }
+        }
+        T* y = reinterpret_cast<T*>(p.y + t * p.y_stride);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (n + q < p.n) y[n + q] = (T)sum[0][q];
+    });
+}
+
+template <typename T, int FM, int FN>
+hipError_t go_few(const Args& p, bool aligned, bool b_aligned, hipStream_t stream) {
+    const dim3 grid((p.n + 16 * FN - 1) / (16 * FN), (p.T + 16 * FM - 1) / (16 * FM));
+    constexpr int lds = stream_lds<FM, FN>();
+    static_assert(lds <= 64 * 1024, "no raised limit needed");
+    if (aligned && b_aligned) project_few_kernel<T, FM, FN, true, true><<<grid, kStreamThreads, lds, stream>>>(p);
+    else if (aligned) project_few_kernel<T, FM, FN, true, false><<<grid, kStreamThreads, lds, stream>>>(p);
+    else if (b_aligned) project_few_kernel<T, FM, FN, false, true><<<grid, kStreamThreads, lds, stream>>>(p);
+    else project_few_kernel<T, FM, FN, false, false><<<grid, kStreamThreads, lds, stream>>>(p);
+    return hipGetLastError();
+}
+
 template <typename T, typename S, bool ALIGNED, bool B_ALIGNED>
 hipError_t go(const Args& p, hipStream_t stream) {
     const long long grid = (long long)((p.T + S::kRows - 1) / S::kRows) * ((p.n + S::kCols - 1) / S::kCols);
@@ -132,9 +248,23 @@ hipError_t go(const Args& p, hipStream_t stream) {
 template <typename T>
 hipError_t run(const Args& p, hipStream_t stream) {
     using S = Shape<1, 4, 4, 2>;
-    shrink_kernel<T><<<p.T, 256, 0, stream>>>(p);
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | p.x_stride | p.d * sizeof(T)) & 15) == 0;
+    const bool a_aligned = aligned && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
     const bool b_aligned = ((reinterpret_cast<uintptr_t>(p.b) | p.r * sizeof(T)) & 15) == 0;
+    if (p.T <= kFewShrink) {
+        const dim3 grid(p.T, (p.u_stride / (int)sizeof(T) + 3) / 4);
+        if (a_aligned) shrink_few_kernel<T, true><<<grid, 256, 0, stream>>>(p);
+        else shrink_few_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+    } else {
+        constexpr int FM = 2, lds = stream_lds<FM, 2>();
+        const dim3 grid((p.T + 16 * FM - 1) / (16 * FM), (p.r + 31) / 32);
+        if (a_aligned) shrink_kernel<T, FM, true><<<grid, kStreamThreads, lds, stream>>>(p);
+        else shrink_kernel<T, FM, false><<<grid, kStreamThreads, lds, stream>>>(p);
+    }
+    const bool wide = p.n >= 32 * 512;  // two workgroups for every compute unit with 32 weight rows each
+    if (p.T <= 16) return wide ? go_few<T, 1, 2>(p, aligned, b_aligned, stream) : go_few<T, 1, 1>(p, aligned, b_aligned, stream);
+    if (p.T <= 32) return wide ? go_few<T, 2, 2>(p, aligned, b_aligned, stream) : go_few<T, 2, 1>(p, aligned, b_aligned, stream);
+    if (p.T <= 64) return wide ? go_few<T, 4, 2>(p, aligned, b_aligned, stream) : go_few<T, 4, 1>(p, aligned, b_aligned, stream);
     if (aligned) return b_aligned ? go<T, S, true, true>(p, stream) : go<T, S, true, false>(p, stream);
     return b_aligned ? go<T, S, false, true>(p, stream) : go<T, S, false, false>(p, stream);
 }

@@ -38,13 +38,22 @@ __device__ __forceinline__ v4f mma(v4u w, v4u x, v4f c, float) {
 }
 
 // 16 bytes of a row from byte k on, zeros from byte `end` on.  ALIGNED: rows start on 16-byte boundaries and `end` is a
-// multiple of 16.
+// multiple of 16.  Otherwise whole pieces are still one load (global memory takes 16 bytes at any address), and only the
+// piece across a row's end is put together from elements.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ v4u whole_piece(const char* at) {
+    if constexpr (ALIGNED) return *reinterpret_cast<const v4u*>(at);
+    v4u v;
+    __builtin_memcpy(&v, at, 16);
+    return v;
+}
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ v4u piece(const char* row, int k, int end) {
     if constexpr (ALIGNED) {
         const v4u v = *reinterpret_cast<const v4u*>(row + min(k, end - 16));
         return k < end ? v : v4u{0, 0, 0, 0};
     } else {
+        if (k + 16 <= end) return whole_piece<T, false>(row + k);
         union {
             T e[16 / sizeof(T)];
             v4u v;
@@ -53,7 +62,7 @@ __device__ __forceinline__ v4u piece(const char* row, int k, int end) {
         const T* p = reinterpret_cast<const T*>(row + k);
         const int left = (end - k) / (int)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < (int)(16 / sizeof(T)); ++i)
+        for (int i = 0; i < (int)(16 / sizeof(T)) - 1; ++i)
             if (i < left) u.e[i] = p[i];
         return u.v;
     }
@@ -82,8 +91,16 @@ __device__ __forceinline__ void walk(char* lds, const char* const (&pa)[S::kPiec
     const int wm = wave / S::WN, wn = wave % S::WN;
     v4u ra[S::kPiecesA], rb[S::kPiecesB];
     const int steps = (end + kStepBytes - 1) / kStepBytes;
+    const int whole = end / kStepBytes;  // steps without a row's end
     auto fetch = [&](int s) {
         const int k = s * kStepBytes + (my_piece << 4);
+        if (s < whole) {
+#pragma unroll
+            for (int i = 0; i < S::kPiecesA; ++i) ra[i] = whole_piece<T, ALIGNED>(pa[i] + k);
+#pragma unroll
+            for (int i = 0; i < S::kPiecesB; ++i) rb[i] = whole_piece<T, ALIGNED>(pb[i] + k);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < S::kPiecesA; ++i) ra[i] = piece<T, ALIGNED>(pa[i], k, end);
 #pragma unroll

@@ -13,43 +13,50 @@ import torch
 from . import capi
 
 _DTYPES = {torch.float32: capi.DTYPE_F32, torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16}
+_F32, _I32 = torch.float32, torch.int32
+_lib = None
 
 
-def _need(cond: bool, message: str) -> None:
-    if not cond:
-        raise capi.InfMoEError(capi.ERR_INVALID_ARGUMENT, message)
+def _load():
+    global _lib
+    _lib = capi.load()
+    return _lib
 
 
-def _dtype(name: str, t: torch.Tensor) -> int:
+def _refuse(message: str) -> None:
+    raise capi.InfMoEError(capi.ERR_INVALID_ARGUMENT, message)
+
+
+def _start(name: str, t: torch.Tensor) -> Tuple[int, int, int, int]:
+    """Checks the operator's matrix of rows; returns (rows, columns, row stride, dtype code)."""
     code = _DTYPES.get(t.dtype)
-    _need(code is not None, f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
-    return code
+    if code is None:
+        _refuse(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+    if not t.is_cuda:
+        _refuse("tensors must be on the GPU")
+    if t.dim() != 2:
+        _refuse(f"{name} must be [rows, columns]")
+    (rows, cols), (stride, step) = t.shape, t.stride()
+    if step != 1 and cols > 1:
+        _refuse(f"{name}: the elements of a row must lie side by side")
+    return rows, cols, stride if rows > 1 else max(cols, 1), code
 
 
-def _rows(name: str, t: torch.Tensor, cols: Optional[int] = None) -> int:
-    """Checks a matrix of rows whose elements lie side by side; returns its row stride."""
-    _need(t.dim() == 2 and (cols is None or t.shape[1] == cols), f"{name} must be [rows, {cols if cols is not None else 'columns'}]")
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: the elements of a row must lie side by side")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+def _check(name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int, ...], device: torch.device) -> None:
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        _refuse(f"{name} must be contiguous {dtype} {list(shape)} on {device}, not {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _same_device(first: torch.Tensor, **tensors: Optional[torch.Tensor]) -> None:
-    _need(first.is_cuda, "tensors must be on the GPU")
-    for name, t in tensors.items():
-        _need(t is None or t.device == first.device, f"{name} is on {None if t is None else t.device}, not on {first.device}")
-
-
-def _on(device: torch.device, call, *args) -> None:
-    """call(*args, stream) with the tensors' device current and its current stream."""
-    if device.index == torch.cuda.current_device():
-        capi.check(call(*args, torch.cuda.current_stream(device).cuda_stream))
+def _call(device: torch.device, function, *args) -> None:
+    """function(*args, stream) with the tensors' device current and its current stream."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            capi.check(call(*args, torch.cuda.current_stream(device).cuda_stream))
-
-
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        capi.check(status)
 
 
 def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
@@ -59,38 +66,44 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Op
 
     score: "softmax" or "sigmoid"; bias: float32 [E], added to the scores for the choice only; groups > 1: only the
     top_groups groups with the largest sums of their group_top best experts stay.  See infmoe_route_topk."""
-    _same_device(logits, bias=bias)
-    dtype, stride = _dtype("logits", logits), _rows("logits", logits)
-    T, E = logits.shape
-    _need(score in capi.SCORE_KINDS, f"unknown score {score!r}")
-    _need(bias is None or (bias.dtype == torch.float32 and bias.shape == (E,) and bias.is_contiguous()), "bias must be float32 [E]")
+    T, E, stride, dtype = _start("logits", logits)
+    device = logits.device
+    kind = capi.SCORE_KINDS.get(score)
+    if kind is None:
+        _refuse(f"unknown score {score!r}")
+    if bias is not None:
+        _check("bias", bias, _F32, (E,), device)
     if out is None:
-        _need(0 < k <= E, "k must be 1 to the number of experts")
-        ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
-        weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+        if not 0 < k <= E:
+            _refuse("k must be 1 to the number of experts")
+        ids = torch.empty((T, k), dtype=_I32, device=device)
+        weights = torch.empty((T, k), dtype=_F32, device=device)
     else:
         ids, weights = out
-        _same_device(logits, ids=ids, weights=weights)
-        _need(ids.dtype == torch.int32 and ids.shape == (T, k) and ids.is_contiguous(), "ids must be a contiguous int32 [T, k]")
-        _need(weights.dtype == torch.float32 and weights.shape == (T, k) and weights.is_contiguous(), "weights must be a contiguous float32 [T, k]")
-    _on(logits.device, capi.load().infmoe_route_topk, T, E, k, dtype, logits.data_ptr(), stride, capi.SCORE_KINDS[score], _ptr(bias),
-        groups, top_groups, group_top, int(renormalize), scale, ids.data_ptr(), weights.data_ptr())
+        _check("ids", ids, _I32, (T, k), device)
+        _check("weights", weights, _F32, (T, k), device)
+    _call(device, (_lib or _load()).infmoe_route_topk, T, E, k, dtype, logits.data_ptr(), stride, kind, None if bias is None else bias.data_ptr(),
+          groups, top_groups, group_top, renormalize, scale, ids.data_ptr(), weights.data_ptr())
     return ids, weights
 
 
-def _matrices(name: str, t: torch.Tensor, like: torch.Tensor, shape: Tuple[int, ...]) -> int:
+def _matrices(name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int, int, int], device: torch.device) -> int:
     """Checks [E, rows, columns] of contiguous matrices; returns the elements from one matrix to the next."""
-    _need(t.dtype == like.dtype, f"{name} must be {like.dtype} as x is, not {t.dtype}")
-    _need(t.dim() == 3 and tuple(t.shape) == shape, f"{name} must be {list(shape)}, not {list(t.shape)}")
-    _need((shape[2] == 1 or t.stride(2) == 1) and (shape[1] == 1 or t.stride(1) == shape[2]), f"{name}: each matrix must be contiguous")
-    return t.stride(0) if shape[0] > 1 else shape[1] * shape[2]
+    E, rows, cols = shape
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
+        _refuse(f"{name} must be {dtype} {list(shape)} on {device}, not {t.dtype} {list(t.shape)} on {t.device}")
+    each, row, step = t.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and row != cols):
+        _refuse(f"{name}: each matrix must be contiguous")
+    return each if E > 1 else rows * cols
 
 
-def _out(name: str, out: Optional[torch.Tensor], x: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+def _out(out: Optional[torch.Tensor], x: torch.Tensor, rows: int, cols: int) -> Tuple[torch.Tensor, int]:
     if out is None:
-        return torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    _need(out.dtype == x.dtype and out.device == x.device and tuple(out.shape) == (rows, cols), f"{name} must be {x.dtype} [{rows}, {cols}] on {x.device}")
-    return out
+        return torch.empty((rows, cols), dtype=x.dtype, device=x.device), cols
+    if out.dtype is not x.dtype or out.device != x.device or out.shape != (rows, cols):
+        _refuse(f"out must be {x.dtype} [{rows}, {cols}] on {x.device}")
+    return out, _start("out", out)[2]
 
 
 def experts_topk(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, wi: torch.Tensor, wo: torch.Tensor,
@@ -100,25 +113,25 @@ def experts_topk(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, wi: 
 
     ffn: "relu", "gated_gelu" or "gated_silu" (the gated ones take wi_1).  An id that is no expert adds nothing.  See
     infmoe_experts_topk."""
-    _same_device(x, ids=ids, weights=weights, wi=wi, wo=wo, wi_1=wi_1)
-    dtype, x_stride = _dtype("x", x), _rows("x", x)
-    _need(ffn in capi.TOPK_FFN_KINDS, f"unknown ffn {ffn!r}")
-    _need((wi_1 is None) == (ffn == "relu"), "wi_1 goes with the gated kinds")
-    T, d = x.shape
-    _need(wi.dim() == 3, "wi must be [E, h, d]")
-    E, h = wi.shape[:2]
-    _need(ids.dim() == 2 and ids.shape[0] == T, "ids must be [T, k]")
-    k = ids.shape[1]
-    _need(ids.dtype == torch.int32 and ids.is_contiguous(), "ids must be contiguous int32 [T, k]")
-    _need(weights.dtype == torch.float32 and weights.shape == ids.shape and weights.is_contiguous(), "weights must be contiguous float32 [T, k]")
-    wi_stride, wo_stride = _matrices("wi", wi, x, (E, h, d)), _matrices("wo", wo, x, (E, d, h))
-    _need(wi_1 is None or _matrices("wi_1", wi_1, x, (E, h, d)) == wi_stride, "wi and wi_1 must be strided alike")
-    y = _out("out", out, x, T, d)
-    y_stride = _rows("out", y)
-    lib = capi.load()
-    ws = torch.empty(lib.infmoe_experts_topk_workspace_bytes(T, k, E, d, h, dtype), dtype=torch.uint8, device=x.device)
-    _on(x.device, lib.infmoe_experts_topk, T, k, E, d, h, capi.TOPK_FFN_KINDS[ffn], dtype, x.data_ptr(), x_stride, ids.data_ptr(),
-        weights.data_ptr(), wi.data_ptr(), _ptr(wi_1), wo.data_ptr(), wi_stride, wo_stride, y.data_ptr(), y_stride, ws.data_ptr())
+    T, d, x_stride, dtype = _start("x", x)
+    device, kind = x.device, capi.TOPK_FFN_KINDS.get(ffn)
+    if kind is None:
+        _refuse(f"unknown ffn {ffn!r}")
+    if (wi_1 is None) != (ffn == "relu"):
+        _refuse("wi_1 goes with the gated kinds")
+    if wi.dim() != 3 or ids.dim() != 2:
+        _refuse("wi must be [E, h, d] and ids [T, k]")
+    E, h, k = wi.shape[0], wi.shape[1], ids.shape[1]
+    _check("ids", ids, _I32, (T, k), device)
+    _check("weights", weights, _F32, (T, k), device)
+    wi_stride, wo_stride = _matrices("wi", wi, x.dtype, (E, h, d), device), _matrices("wo", wo, x.dtype, (E, d, h), device)
+    if wi_1 is not None and _matrices("wi_1", wi_1, x.dtype, (E, h, d), device) != wi_stride:
+        _refuse("wi and wi_1 must be strided alike")
+    y, y_stride = _out(out, x, T, d)
+    lib = _lib or _load()
+    ws = torch.empty(lib.infmoe_experts_topk_workspace_bytes(T, k, E, d, h, dtype), dtype=torch.uint8, device=device)
+    _call(device, lib.infmoe_experts_topk, T, k, E, d, h, kind, dtype, x.data_ptr(), x_stride, ids.data_ptr(), weights.data_ptr(), wi.data_ptr(),
+          None if wi_1 is None else wi_1.data_ptr(), wo.data_ptr(), wi_stride, wo_stride, y.data_ptr(), y_stride, ws.data_ptr())
     return y
 
 
@@ -126,20 +139,20 @@ def lora_project(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Ten
                  scale: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] = w x[t] + scale[i] * b[i] (a[i] x[t]) with i = adapter[t]: x [T, d], w [n, d], a [L, r, d], b [L, n, r], adapter int32
     [T], scale float32 [L] -> [T, n].  A row whose adapter is none of the L gets w x[t].  See infmoe_lora_project."""
-    _same_device(x, w=w, a=a, b=b, adapter=adapter, scale=scale)
-    dtype, x_stride = _dtype("x", x), _rows("x", x)
-    T, d = x.shape
-    _need(w.dtype == x.dtype and w.dim() == 2 and w.shape[1] == d and w.is_contiguous(), f"w must be contiguous {x.dtype} [n, {d}]")
-    n = w.shape[0]
-    _need(a.dim() == 3 and a.is_contiguous() and b.is_contiguous(), "a and b must be contiguous [L, r, d] and [L, n, r]")
-    L, r = a.shape[:2]
-    _matrices("a", a, x, (L, r, d)), _matrices("b", b, x, (L, n, r))
-    _need(adapter.dtype == torch.int32 and adapter.shape == (T,) and adapter.is_contiguous(), "adapter must be contiguous int32 [T]")
-    _need(scale is None or (scale.dtype == torch.float32 and scale.shape == (L,) and scale.is_contiguous()), "scale must be float32 [L]")
-    y = _out("out", out, x, T, n)
-    y_stride = _rows("out", y)
-    lib = capi.load()
-    ws = torch.empty(lib.infmoe_lora_project_workspace_bytes(T, d, n, r, dtype), dtype=torch.uint8, device=x.device)
-    _on(x.device, lib.infmoe_lora_project, T, d, n, r, L, dtype, x.data_ptr(), x_stride, w.data_ptr(), a.data_ptr(), b.data_ptr(),
-        adapter.data_ptr(), _ptr(scale), y.data_ptr(), y_stride, ws.data_ptr())
+    T, d, x_stride, dtype = _start("x", x)
+    device = x.device
+    if w.dim() != 2 or a.dim() != 3:
+        _refuse("w must be [n, d] and a [L, r, d]")
+    n, (L, r) = w.shape[0], a.shape[:2]
+    _check("w", w, x.dtype, (n, d), device)
+    _check("a", a, x.dtype, (L, r, d), device)
+    _check("b", b, x.dtype, (L, n, r), device)
+    _check("adapter", adapter, _I32, (T,), device)
+    if scale is not None:
+        _check("scale", scale, _F32, (L,), device)
+    y, y_stride = _out(out, x, T, n)
+    lib = _lib or _load()
+    ws = torch.empty(lib.infmoe_lora_project_workspace_bytes(T, d, n, r, dtype), dtype=torch.uint8, device=device)
+    _call(device, lib.infmoe_lora_project, T, d, n, r, L, dtype, x.data_ptr(), x_stride, w.data_ptr(), a.data_ptr(), b.data_ptr(), adapter.data_ptr(),
+          None if scale is None else scale.data_ptr(), y.data_ptr(), y_stride, ws.data_ptr())
     return y
