@@ -14,6 +14,7 @@
 #include "kernels.h"
 #include "row_gemm.h"
 #include "row_stream.h"
+#include "row_tall.h"
 
 namespace infmoe {
 namespace {
@@ -109,7 +110,10 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(int S, int E, co
         const int mine = (count + tile_rows - 1) / tile_rows;
         int n = 0;
         const int first = block_prefix(mine, s_wave, &n);
-        for (int j = 0; j < mine; ++j) tiles[first + j] = int4{i, offset + j * tile_rows, min(tile_rows, count - j * tile_rows), 0};
+        // as few tiles as the height allows, of one height (a multiple of 32 where tiles are that tall)
+        const int even = mine > 1 ? (count + mine - 1) / mine : tile_rows;
+        const int height = tile_rows > 64 ? (even + 31) / 32 * 32 : tile_rows;
+        for (int j = 0; j < mine; ++j) tiles[first + j] = int4{i, offset + j * height, min(height, count - j * height), 0};
         if (i == 0) *n_tiles = n;
     }
     __syncthreads();
@@ -178,6 +182,66 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Product p) {
                     static_cast<float*>(p.c)[(size_t)p.row_slot[row] * p.N + n + q] = acc[i][j][q];
             }
         }
+    }
+}
+
+// ---- many rows per expert (row_tall.h).  The height of a tile is a run-time multiple of 32 rows.
+template <typename T, int FM, bool FIRST, bool GATED>
+__device__ __forceinline__ void tall_body(const Product& p, const int4& tile, int n0, char* lds) {
+    constexpr int F = GATED ? 2 : 4, kWaveCols = 16 * F;
+    using W = Tall<FM, F>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+    const int row_bytes = p.K * (int)sizeof(T);
+    const char *pa[W::kPiecesA], *pb[2];
+#pragma unroll
+    for (int i = 0; i < W::kPiecesA; ++i) {
+        const int r = tile.y + min(W::row_a(i), tile.z - 1);
+        pa[i] = p.a + (FIRST ? (long long)(p.row_slot[r] / p.k_slots) : (long long)r) * p.a_stride + W::byte_a();
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int v = W::row_b(i), q = v & 63, n = n0 + (v >> 6) * kWaveCols + q % kWaveCols;
+        pb[i] = (q >= kWaveCols ? p.b1 : p.b) + tile.x * p.b_expert + (long long)min(n, p.N - 1) * row_bytes + W::byte_b(i);
+    }
+    v4f acc[FM][4];
+    tall_multiply<T, FM, F>(acc, lds, pa, pb, row_bytes);
+    const bool whole = p.N % (16 / (FIRST ? (int)sizeof(T) : 4)) == 0;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int r = (wm * FM + i) * 16 + (lane & 15);
+        if (r >= tile.z) continue;
+        const int row = tile.y + r, n = n0 + wn * kWaveCols + W::column();
+        if constexpr (FIRST)
+            write_columns<T, 4 * F>(static_cast<T*>(p.c) + (size_t)row * p.N, n, p.N, whole, [&](int c) {
+                return activate<T>(p.ffn, acc[i][c >> 2][c & 3], GATED ? acc[i][(c >> 2) + 4 - F][c & 3] : 0.f);
+            });
+        else
+            write_columns<float, 4 * F>(static_cast<float*>(p.c) + (size_t)p.row_slot[row] * p.N, n, p.N, whole,
+                                        [&](int c) { return acc[i][c >> 2][c & 3]; });
+    }
+}
+
+template <typename T, bool FIRST, bool GATED>
+__global__ __launch_bounds__(kTallThreads) void tall_kernel(Product p) {
+    extern __shared__ __align__(16) char lds[];
+    constexpr int kOut = GATED ? kTallCols / 2 : kTallCols;
+    const int cols = (p.N + kOut - 1) / kOut;
+    // Workgroups are dealt to the dies in turn; each die takes a contiguous stretch of (tile, column) pairs, so that those
+    // at work in one die at a time share a tile's rows in its L2.  The tiles that exist are fewer than the grid has room for.
+    const int n = *p.n_tiles * cols, share = (n + kXcdCount - 1) / kXcdCount;
+    const int mine = blockIdx.x / kXcdCount, id = (blockIdx.x % kXcdCount) * share + mine;
+    if (mine >= share || id >= n) return;
+    const int4 tile = p.tiles[id / cols];
+    const int n0 = id % cols * kOut;
+    switch ((tile.z + 31) / 32) {
+        case 1:
+        case 2: tall_body<T, 2, FIRST, GATED>(p, tile, n0, lds); break;
+        case 3: tall_body<T, 3, FIRST, GATED>(p, tile, n0, lds); break;
+        case 4: tall_body<T, 4, FIRST, GATED>(p, tile, n0, lds); break;
+        case 5: tall_body<T, 5, FIRST, GATED>(p, tile, n0, lds); break;
+        case 6: tall_body<T, 6, FIRST, GATED>(p, tile, n0, lds); break;
+        case 7: tall_body<T, 7, FIRST, GATED>(p, tile, n0, lds); break;
+        default: tall_body<T, 8, FIRST, GATED>(p, tile, n0, lds); break;
     }
 }
 
@@ -322,6 +386,16 @@ hipError_t go(const Product& p, int max_tiles, bool aligned, hipStream_t stream)
     return hipGetLastError();
 }
 
+template <typename T, bool FIRST, bool GATED>
+hipError_t go_tall(const Product& p, int max_tiles, hipStream_t stream) {
+    constexpr int out = GATED ? kTallCols / 2 : kTallCols;
+    const long long grid = ((long long)max_tiles * ((p.N + out - 1) / out) + kXcdCount - 1) / kXcdCount * kXcdCount;
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    if (const hipError_t err = allow_lds_once<tall_kernel<T, FIRST, GATED>>(kTallLds); err != hipSuccess) return err;
+    tall_kernel<T, FIRST, GATED><<<(int)grid, kTallThreads, kTallLds, stream>>>(p);
+    return hipGetLastError();
+}
+
 template <typename T, int FM, int FN, bool FIRST, bool GATED>
 hipError_t go_stream(const Product& p, const FewRows& few, int max_tiles, bool aligned, hipStream_t stream) {
     constexpr int out = 16 * FN / (GATED ? 2 : 1), lds = stream_lds<FM, FN>();
@@ -357,7 +431,12 @@ hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long lon
     // few rows per expert: tiles of 16 or 32 rows, weights streamed
     const int few_blocks = slots <= 4 * E ? 1 : slots <= 16 * E ? 2 : 0;
     const bool mini = few_blocks > 0 && slots <= kMiniSlots;
-    const int tile_rows = few_blocks > 0 ? 16 * few_blocks : S::kRows;
+    auto on16 = [](const void* p, long long stride) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (long long)sizeof(T))) & 15) == 0; };
+    const bool in_ok = d * sizeof(T) % 16 == 0 && on16(x, x_stride) && on16(wi, wi_stride) && on16(wi_1, 0);
+    const bool out_ok = h * sizeof(T) % 16 == 0 && on16(wo, wo_stride);
+    const bool tall = few_blocks == 0 && in_ok && out_ok &&
+                      (slots / kTallRows + std::min(E, slots) / 2) * (long long)((std::min(d, h) + kTallCols - 1) / kTallCols) >= 200;
+    const int tile_rows = few_blocks > 0 ? 16 * few_blocks : tall ? kTallRows : S::kRows;
     if (!mini) {
         if (blocks > 1) plan_count_kernel<<<blocks, kPlanBlock, 4 * E, stream>>>(slots, E, ids, c.hist);
         const size_t lds = 4 * (size_t)kPlanWaves * E;
@@ -365,30 +444,30 @@ hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long lon
         plan_place_kernel<<<blocks, kPlanBlock, lds, stream>>>(slots, E, ids, blocks > 1 ? c.hist : nullptr, tile_rows, c.row_slot, c.tiles, c.n_tiles);
     }
     const int max_tiles = (mini ? 0 : slots / tile_rows) + std::min(E, slots);
-    auto on16 = [](const void* p, long long stride) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (long long)sizeof(T))) & 15) == 0; };
     const FewRows few{mini ? ids : nullptr, slots, E};
     Product p{};
     p.row_slot = c.row_slot, p.tiles = c.tiles, p.n_tiles = c.n_tiles, p.k_slots = k, p.ffn = ffn;
     p.a = reinterpret_cast<const char*>(x), p.a_stride = x_stride * sizeof(T);
     p.b = reinterpret_cast<const char*>(wi), p.b1 = reinterpret_cast<const char*>(wi_1), p.b_expert = wi_stride * sizeof(T);
     p.c = c.hidden, p.N = h, p.K = d;
-    const bool in_ok = d * sizeof(T) % 16 == 0 && on16(x, x_stride) && on16(wi, wi_stride) && on16(wi_1, 0);
     hipError_t err;
     if (ffn == FFN_RELU)
         err = few_blocks == 1   ? go_few<T, 1, true, false>(p, few, max_tiles, in_ok, stream)
               : few_blocks == 2 ? go_few<T, 2, true, false>(p, few, max_tiles, in_ok, stream)
+              : tall            ? go_tall<T, true, false>(p, max_tiles, stream)
                                 : go<T, S, true, false>(p, max_tiles, in_ok, stream);
     else
         err = few_blocks == 1   ? go_few<T, 1, true, true>(p, few, max_tiles, in_ok, stream)
               : few_blocks == 2 ? go_few<T, 2, true, true>(p, few, max_tiles, in_ok, stream)
+              : tall            ? go_tall<T, true, true>(p, max_tiles, stream)
                                 : go<T, S, true, true>(p, max_tiles, in_ok, stream);
     if (err != hipSuccess) return err;
     p.a = c.hidden, p.a_stride = (long long)h * sizeof(T);
     p.b = reinterpret_cast<const char*>(wo), p.b1 = nullptr, p.b_expert = wo_stride * sizeof(T);
     p.c = c.post, p.N = d, p.K = h;
-    const bool out_ok = h * sizeof(T) % 16 == 0 && on16(wo, wo_stride);
     err = few_blocks == 1   ? go_few<T, 1, false, false>(p, few, max_tiles, out_ok, stream)
           : few_blocks == 2 ? go_few<T, 2, false, false>(p, few, max_tiles, out_ok, stream)
+          : tall            ? go_tall<T, false, false>(p, max_tiles, stream)
                             : go<T, S, false, false>(p, max_tiles, out_ok, stream);
     if (err != hipSuccess) return err;
     combine_kernel<T><<<dim3(Tn, (d + 1023) / 1024), 256, 0, stream>>>(d, k, E, ids, weights, c.post, y, y_stride);

@@ -9,6 +9,7 @@
 #include "kernels.h"
 #include "row_gemm.h"
 #include "row_stream.h"
+#include "row_tall.h"
 
 namespace infmoe {
 namespace {
@@ -185,6 +186,95 @@ __global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
     }
 }
 
+// Many rows: tiles of 32 * FM x 256 (row_tall.h).  The adapters' part needs no LDS and no barrier: every wave goes over the
+// adapters among its own 16 * FM rows and takes u and B_a from the caches straight into operands.
+constexpr int kTileGroup = 4;  // row tiles that share a stretch of weight columns (below)
+
+template <typename T, int FM, bool B_ALIGNED>
+__global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
+    extern __shared__ __align__(16) char lds[];
+    using W = Tall<FM, 4>;
+    constexpr int kRows = 32 * FM;
+    const int cols = (p.n + kTallCols - 1) / kTallCols, tiles = (p.T + kRows - 1) / kRows;
+    // Workgroups are dealt to the dies in turn; each die takes a contiguous stretch of tiles, walked kTileGroup row tiles by
+    // one column tile at a time: those at work in a die at one time share a few row and column tiles in its L2.
+    const int share = (tiles * cols + kXcdCount - 1) / kXcdCount, id = (int)(blockIdx.x % kXcdCount) * share + (int)(blockIdx.x / kXcdCount);
+    if ((int)(blockIdx.x / kXcdCount) >= share || id >= tiles * cols) return;
+    const int band = id / (kTileGroup * cols), in_band = id % (kTileGroup * cols), high = min(kTileGroup, tiles - band * kTileGroup);
+    const int row0 = (band * kTileGroup + in_band % high) * kRows, n0 = in_band / high * kTallCols;
+    const int count = min(kRows, p.T - row0);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+    const int end = p.d * (int)sizeof(T);
+    const char *pa[W::kPiecesA], *pb[2];
+#pragma unroll
+    for (int i = 0; i < W::kPiecesA; ++i) pa[i] = p.x + (row0 + min(W::row_a(i), count - 1)) * p.x_stride + W::byte_a();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pb[i] = p.w + (long long)min(n0 + W::row_b(i), p.n - 1) * end + W::byte_b(i);
+    v4f acc[FM][4];
+    tall_multiply<T, FM, 4>(acc, lds, pa, pb, end);
+
+    const int m = lane & 15, r_end = p.r * (int)sizeof(T);
+    int mine[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int r = (wm * FM + i) * 16 + m;
+        mine[i] = r < count ? p.adapter[row0 + r] : -1;
+        if (mine[i] >= p.L) mine[i] = -1;
+    }
+    for (;;) {
+        int a = -1;  // the first adapter that is left (rows that have been served get -1)
+#pragma unroll
+        for (int i = FM - 1; i >= 0; --i) {
+            const unsigned long long left = __ballot(mine[i] >= 0);
+            if (left != 0) a = __builtin_amdgcn_readlane(mine[i], __ffsll((long long)left) - 1);
+        }
+        if (a < 0) break;
+        const char* pw[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = n0 + wn * 64 + (m >> 2) * 16 + 4 * j + (m & 3);
+            pw[j] = p.b + ((long long)a * p.n + min(n, p.n - 1)) * r_end;
+        }
+        for (int k = (lane >> 4) * 16; k - (lane >> 4) * 16 < r_end; k += 64) {
+            v4u wb[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wb[j] = k < r_end ? piece<T, B_ALIGNED>(pw[j], k, r_end) : v4u{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                if (__ballot(mine[i] == a) == 0) continue;
+                const size_t row = row0 + min((wm * FM + i) * 16 + m, count - 1);
+                const v4u u = piece<T, true>(p.u + row * p.u_stride, k, p.u_stride);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    // a sum of its own: what another adapter's rows and weights hold (infinities, NaN) stays out of acc
+                    const v4f sum = mma(wb[j], u, v4f{0.f, 0.f, 0.f, 0.f}, T{});
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[i][j][q] += mine[i] == a ? sum[q] : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) mine[i] = mine[i] == a ? -1 : mine[i];
+    }
+    const bool whole = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.y_stride) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int r = (wm * FM + i) * 16 + m;
+        if (r < count)
+            write_columns<T, 16>(reinterpret_cast<T*>(p.y + (row0 + r) * p.y_stride), n0 + wn * 64 + W::column(), p.n, whole,
+                                 [&](int c) { return acc[i][c >> 2][c & 3]; });
+    }
+}
+
+template <typename T, int FM, bool B_ALIGNED>
+hipError_t go_tall(const Args& p, hipStream_t stream) {
+    const long long all = (long long)((p.T + 32 * FM - 1) / (32 * FM)) * ((p.n + kTallCols - 1) / kTallCols);
+    if (all > 0x7ffffff0) return hipErrorInvalidValue;
+    if (const hipError_t err = allow_lds_once<project_tall_kernel<T, FM, B_ALIGNED>>(kTallLds); err != hipSuccess) return err;
+    project_tall_kernel<T, FM, B_ALIGNED><<<(int)((all + kXcdCount - 1) / kXcdCount * kXcdCount), kTallThreads, kTallLds, stream>>>(p);
+    return hipGetLastError();
+}
+
 // Few rows: W streamed once through the registers, 16 * FN of its rows per workgroup; the adapters' part of an output is added
 // by the lane that holds the joined sum.
 template <typename T, int FM, int FN, bool ALIGNED, bool B_ALIGNED>
@@ -265,6 +355,10 @@ hipError_t run(const Args& p, hipStream_t stream) {
     if (p.T <= 16) return wide ? go_few<T, 1, 2>(p, aligned, b_aligned, stream) : go_few<T, 1, 1>(p, aligned, b_aligned, stream);
     if (p.T <= 32) return wide ? go_few<T, 2, 2>(p, aligned, b_aligned, stream) : go_few<T, 2, 1>(p, aligned, b_aligned, stream);
     if (p.T <= 64) return wide ? go_few<T, 4, 2>(p, aligned, b_aligned, stream) : go_few<T, 4, 1>(p, aligned, b_aligned, stream);
+    // tall tiles where there are enough of them for the compute units
+    const long long columns = (p.n + kTallCols - 1) / kTallCols;
+    if (aligned && (p.T + 255) / 256 * columns >= 200) return b_aligned ? go_tall<T, 8, true>(p, stream) : go_tall<T, 8, false>(p, stream);
+    if (aligned && (p.T + 127) / 128 * columns >= 100) return b_aligned ? go_tall<T, 4, true>(p, stream) : go_tall<T, 4, false>(p, stream);
     if (aligned) return b_aligned ? go<T, S, true, true>(p, stream) : go<T, S, true, false>(p, stream);
     return b_aligned ? go<T, S, false, true>(p, stream) : go<T, S, false, false>(p, stream);
 }

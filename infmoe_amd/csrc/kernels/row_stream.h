@@ -8,8 +8,6 @@
 // 16 rows, because lanes past the last row repeat its address).
 #pragma once
 
-#include <type_traits>
-
 #include "row_gemm.h"
 
 namespace infmoe {
