@@ -192,14 +192,14 @@ __device__ __forceinline__ void tall_body(const Product& p, const int4& tile, in
     using W = Tall<FM, F>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
     const int row_bytes = p.K * (int)sizeof(T);
-    const char *pa[W::kPiecesA], *pb[2];
+    const char *pa[W::kPiecesA], *pb[4];
 #pragma unroll
     for (int i = 0; i < W::kPiecesA; ++i) {
         const int r = tile.y + min(W::row_a(i), tile.z - 1);
-        pa[i] = p.a + (FIRST ? (long long)(p.row_slot[r] / p.k_slots) : (long long)r) * p.a_stride + W::byte_a();
+        pa[i] = p.a + (FIRST ? (long long)(p.row_slot[r] / p.k_slots) : (long long)r) * p.a_stride + W::byte_a(i);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const int v = W::row_b(i), q = v & 63, n = n0 + (v >> 6) * kWaveCols + q % kWaveCols;
         pb[i] = (q >= kWaveCols ? p.b1 : p.b) + tile.x * p.b_expert + (long long)min(n, p.N - 1) * row_bytes + W::byte_b(i);
     }

@@ -205,11 +205,11 @@ __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
     const int count = min(kRows, p.T - row0);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
     const int end = p.d * (int)sizeof(T);
-    const char *pa[W::kPiecesA], *pb[2];
+    const char *pa[W::kPiecesA], *pb[4];
 #pragma unroll
-    for (int i = 0; i < W::kPiecesA; ++i) pa[i] = p.x + (row0 + min(W::row_a(i), count - 1)) * p.x_stride + W::byte_a();
+    for (int i = 0; i < W::kPiecesA; ++i) pa[i] = p.x + (row0 + min(W::row_a(i), count - 1)) * p.x_stride + W::byte_a(i);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) pb[i] = p.w + (long long)min(n0 + W::row_b(i), p.n - 1) * end + W::byte_b(i);
+    for (int i = 0; i < 4; ++i) pb[i] = p.w + (long long)min(n0 + W::row_b(i), p.n - 1) * end + W::byte_b(i);
     v4f acc[FM][4];
     tall_multiply<T, FM, 4>(acc, lds, pa, pb, end);
 
