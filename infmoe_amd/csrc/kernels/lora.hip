@@ -16,7 +16,7 @@ namespace {
 
 using namespace rows;
 
-constexpr int kFewShrink = 256;  // rows up to which u takes a wave per row and rank
+constexpr int kFewShrink = 1024;  // rows up to which u takes waves of their own per row
 
 struct Args {
     const char *x, *w, *a, *b;
@@ -44,28 +44,47 @@ __device__ __forceinline__ float dot_piece(v4u a, v4u b, float sum) {
     return sum;
 }
 
-// u of few rows: a wave per row and rank.
-template <typename T, bool ALIGNED>
+// u of few rows: a wave per row and RJ ranks (one where rows are so few that the waves are wanted, else four, which share the
+// row of x).
+template <typename T, int RJ, bool ALIGNED>
 __global__ __launch_bounds__(256) void shrink_few_kernel(Args p) {
-    const int t = blockIdx.x, lane = threadIdx.x & 63, j = blockIdx.y * 4 + (threadIdx.x >> 6);
-    const int a = p.adapter[t];
-    if (a < 0 || a >= p.L || j >= p.u_stride / (int)sizeof(T)) return;  // (a row without an adapter: its u is never used)
-    float sum = 0.f;
-    if (j < p.r) {
-        const int end = p.d * (int)sizeof(T);
-        const char *x = p.x + t * p.x_stride, *m = p.a + ((long long)a * p.r + j) * end;
-        int k = lane * 16;
-        for (; k + 3 * 1024 + 16 <= end; k += 4 * 1024) {
-            v4u q[4], w[4];
+    const int t = blockIdx.x, lane = threadIdx.x & 63, j0 = (blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RJ;
+    const int a = p.adapter[t], padded = p.u_stride / (int)sizeof(T);
+    if (a < 0 || a >= p.L || j0 >= padded) return;  // (a row without an adapter: its u is never used)
+    const int end = p.d * (int)sizeof(T);
+    const char *x = p.x + t * p.x_stride, *m[RJ];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = whole_piece<T, ALIGNED>(x + k + i * 1024), w[i] = whole_piece<T, ALIGNED>(m + k + i * 1024);
+    for (int q = 0; q < RJ; ++q) m[q] = p.a + ((long long)a * p.r + min(j0 + q, p.r - 1)) * end;
+    float sum[RJ];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum = dot_piece<T>(q[i], w[i], sum);
+    for (int q = 0; q < RJ; ++q) sum[q] = 0.f;
+    constexpr int kLoads = RJ == 1 ? 4 : 2;  // pieces of a row in flight
+    int k = lane * 16;
+    for (; k + (kLoads - 1) * 1024 + 16 <= end; k += kLoads * 1024) {
+        v4u v[kLoads], w[RJ][kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            v[i] = whole_piece<T, ALIGNED>(x + k + i * 1024);
+#pragma unroll
+            for (int q = 0; q < RJ; ++q) w[q][i] = whole_piece<T, ALIGNED>(m[q] + k + i * 1024);
         }
-        for (; k < end; k += 1024) sum = dot_piece<T>(piece<T, ALIGNED>(x, k, end), piece<T, ALIGNED>(m, k, end), sum);
-        sum = wave_sum(sum) * (p.scale != nullptr ? p.scale[a] : 1.f);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+            for (int q = 0; q < RJ; ++q) sum[q] = dot_piece<T>(v[i], w[q][i], sum[q]);
     }
-    if (lane == 0) reinterpret_cast<T*>(p.u + (size_t)t * p.u_stride)[j] = (T)sum;
+    for (; k < end; k += 1024) {
+        const v4u v = piece<T, ALIGNED>(x, k, end);
+#pragma unroll
+        for (int q = 0; q < RJ; ++q) sum[q] = dot_piece<T>(v, piece<T, ALIGNED>(m[q], k, end), sum[q]);
+    }
+    const float s = p.scale != nullptr ? p.scale[a] : 1.f;
+    T* u = reinterpret_cast<T*>(p.u + (size_t)t * p.u_stride);
+#pragma unroll
+    for (int q = 0; q < RJ; ++q) {
+        const float total = wave_sum(sum[q]) * s;
+        if (lane == 0 && j0 + q < padded) u[j0 + q] = (T)(j0 + q < p.r ? total : 0.f);
+    }
 }
 
 // u of many rows: 16 * FM rows of a workgroup against the adapters that occur among them, 32 ranks at a time, on the matrix
@@ -318,12 +337,16 @@ template <typename T, int FM, int FN>
 hipError_t go_few(const Args& p, bool aligned, bool b_aligned, hipStream_t stream) {
     const dim3 grid((p.n + 16 * FN - 1) / (16 * FN), (p.T + 16 * FM - 1) / (16 * FM));
     constexpr int lds = stream_lds<FM, FN>();
-    static_assert(lds <= 64 * 1024, "no raised limit needed");
-    if (aligned && b_aligned) project_few_kernel<T, FM, FN, true, true><<<grid, kStreamThreads, lds, stream>>>(p);
-    else if (aligned) project_few_kernel<T, FM, FN, true, false><<<grid, kStreamThreads, lds, stream>>>(p);
-    else if (b_aligned) project_few_kernel<T, FM, FN, false, true><<<grid, kStreamThreads, lds, stream>>>(p);
-    else project_few_kernel<T, FM, FN, false, false><<<grid, kStreamThreads, lds, stream>>>(p);
-    return hipGetLastError();
+    auto launch = [&](auto kernel) {
+        constexpr auto k = decltype(kernel)::value;
+        if (const hipError_t err = allow_lds_once<k>(lds); err != hipSuccess) return err;
+        k<<<grid, kStreamThreads, lds, stream>>>(p);
+        return hipGetLastError();
+    };
+    if (aligned && b_aligned) return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, true, true>>{});
+    if (aligned) return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, true, false>>{});
+    if (b_aligned) return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, false, true>>{});
+    return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, false, false>>{});
 }
 
 template <typename T, typename S, bool ALIGNED, bool B_ALIGNED>
@@ -341,24 +364,35 @@ hipError_t run(const Args& p, hipStream_t stream) {
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | p.x_stride | p.d * sizeof(T)) & 15) == 0;
     const bool a_aligned = aligned && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
     const bool b_aligned = ((reinterpret_cast<uintptr_t>(p.b) | p.r * sizeof(T)) & 15) == 0;
-    if (p.T <= kFewShrink) {
-        const dim3 grid(p.T, (p.u_stride / (int)sizeof(T) + 3) / 4);
-        if (a_aligned) shrink_few_kernel<T, true><<<grid, 256, 0, stream>>>(p);
-        else shrink_few_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+    const int padded = p.u_stride / (int)sizeof(T);
+    if ((long long)p.T * padded <= 4096) {
+        const dim3 grid(p.T, (padded + 3) / 4);
+        if (a_aligned) shrink_few_kernel<T, 1, true><<<grid, 256, 0, stream>>>(p);
+        else shrink_few_kernel<T, 1, false><<<grid, 256, 0, stream>>>(p);
+    } else if (p.T <= kFewShrink) {
+        const dim3 grid(p.T, (padded + 15) / 16);
+        if (a_aligned) shrink_few_kernel<T, 4, true><<<grid, 256, 0, stream>>>(p);
+        else shrink_few_kernel<T, 4, false><<<grid, 256, 0, stream>>>(p);
     } else {
         constexpr int FM = 2, lds = stream_lds<FM, 2>();
         const dim3 grid((p.T + 16 * FM - 1) / (16 * FM), (p.r + 31) / 32);
         if (a_aligned) shrink_kernel<T, FM, true><<<grid, kStreamThreads, lds, stream>>>(p);
         else shrink_kernel<T, FM, false><<<grid, kStreamThreads, lds, stream>>>(p);
     }
-    const bool wide = p.n >= 32 * 512;  // two workgroups for every compute unit with 32 weight rows each
-    if (p.T <= 16) return wide ? go_few<T, 1, 2>(p, aligned, b_aligned, stream) : go_few<T, 1, 1>(p, aligned, b_aligned, stream);
-    if (p.T <= 32) return wide ? go_few<T, 2, 2>(p, aligned, b_aligned, stream) : go_few<T, 2, 1>(p, aligned, b_aligned, stream);
-    if (p.T <= 64) return wide ? go_few<T, 4, 2>(p, aligned, b_aligned, stream) : go_few<T, 4, 1>(p, aligned, b_aligned, stream);
     // tall tiles where there are enough of them for the compute units
     const long long columns = (p.n + kTallCols - 1) / kTallCols;
     if (aligned && (p.T + 255) / 256 * columns >= 200) return b_aligned ? go_tall<T, 8, true>(p, stream) : go_tall<T, 8, false>(p, stream);
     if (aligned && (p.T + 127) / 128 * columns >= 100) return b_aligned ? go_tall<T, 4, true>(p, stream) : go_tall<T, 4, false>(p, stream);
+    // Streams of up to 64 rows: W passes once per 64 rows.  The rows come through the caches, FM / FN of the weights' bytes,
+    // so as many weight rows per workgroup as leave at least 128 workgroups (64 rows by 10240 x 4096: 16 weight rows 64 us,
+    // 64 of them 26).  With more rows, as long as tiles of 64 x 128 would leave compute units without work.
+    const long long row_tiles = (p.T + 63) / 64;
+    if (p.T <= 16) return p.n >= 32 * 512 ? go_few<T, 1, 2>(p, aligned, b_aligned, stream) : go_few<T, 1, 1>(p, aligned, b_aligned, stream);
+    if (p.T <= 32) return p.n >= 32 * 128 ? go_few<T, 2, 2>(p, aligned, b_aligned, stream) : go_few<T, 2, 1>(p, aligned, b_aligned, stream);
+    if (p.T <= 64 || row_tiles * ((p.n + 127) / 128) < 256) {
+        if (row_tiles * ((p.n + 63) / 64) >= 128) return go_few<T, 4, 4>(p, aligned, b_aligned, stream);
+        return row_tiles * ((p.n + 31) / 32) >= 128 ? go_few<T, 4, 2>(p, aligned, b_aligned, stream) : go_few<T, 4, 1>(p, aligned, b_aligned, stream);
+    }
     if (aligned) return b_aligned ? go<T, S, true, true>(p, stream) : go<T, S, true, false>(p, stream);
     return b_aligned ? go<T, S, false, true>(p, stream) : go<T, S, false, false>(p, stream);
 }

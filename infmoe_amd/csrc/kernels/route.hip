@@ -9,10 +9,14 @@
 // in FP32, and a row in which two neighbours of the ranking are closer than what FP32 can order (see kScoreError) is
 // chosen once more on scores in 64 bits; a result never depends on FP32's roundings.
 //
-// Layout: a row of E logits takes 16, 32 or 64 neighbouring lanes of a wave, each with V <= 32 consecutive experts in
-// registers; a group of experts takes a power of two of those lanes (slots that this leaves over hold minus infinity).
-// Consecutive experts sit in ascending lanes and slots, so "the lowest index" is "the first lane, then the first slot",
-// and all exchanges are between registers of one wave: no LDS, no barrier.
+// Layout: a row of E logits takes a whole wave, or 16 neighbouring lanes of it when it has at most 64 experts, each lane with
+// V <= 32 consecutive experts in registers; a group of experts takes a power of two of those lanes (slots that this leaves
+// over hold minus infinity).  Consecutive experts sit in ascending lanes and slots, so "the lowest index" is "the first
+// lane, then the first slot", and all exchanges are between registers of one wave: no barrier.
+//
+// Bound by vector instructions (131071 rows of 256 experts are 134 MB, 27 us of memory time): a round of the selection is a
+// maximum over the row and the removal of its place.  With a row per wave that place is scalar arithmetic on the masks of
+// V comparisons; with rows of 16 lanes the same instructions serve four rows.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -36,28 +40,43 @@ struct Args {
     float scale;
 };
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+// v of the lane that the data-parallel control names; `other` in the lanes of rows that ROWS leaves out
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float v, float other = 0.f) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, ROWS, 0xf, false));
 }
-template <int CTRL>
-__device__ __forceinline__ double dpp(double v) {
-    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, false);
-    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, false), lo);
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp(double v, double other = 0.0) {
+    const int lo = __builtin_amdgcn_update_dpp(__double2loint(other), __double2loint(v), CTRL, ROWS, 0xf, false);
+    return __hiloint2double(__builtin_amdgcn_update_dpp(__double2hiint(other), __double2hiint(v), CTRL, ROWS, 0xf, false), lo);
 }
-__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ float size_of(float v) { return __builtin_fabsf(v); }
+__device__ __forceinline__ double size_of(double v) { return __builtin_fabs(v); }
 
-// Reductions over the G lanes of a row, the result in all of them.  Inside 16 lanes by data-parallel moves (lane ^ 1,
-// lane ^ 2, mirror in 8, mirror in 16), beyond by two exchanges through the LDS crossbar.
+// lane 63's value in all lanes, as a scalar
+__device__ __forceinline__ float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ double last_lane(double v) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+__device__ __forceinline__ float lane_value(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+
+// Reductions over the G lanes of a row, the result in all of them: lane ^ 1, lane ^ 2, mirror in 8, mirror in 16; over 64
+// lanes then the last lane of 16 to the next 16, and of 32 to the next 32 (the full sums and maxima arrive in lane 63).
 template <int G, typename R>
 __device__ __forceinline__ R row_max(R v) {
     v = larger(v, dpp<0xB1>(v));
     v = larger(v, dpp<0x4E>(v));
     v = larger(v, dpp<0x141>(v));
     v = larger(v, dpp<0x140>(v));
-    if (G > 16) v = larger(v, __shfl_xor(v, 16));
-    if (G > 32) v = larger(v, __shfl_xor(v, 32));
+    if constexpr (G == 64) {
+        v = larger(v, dpp<0x142, 0xa>(v, v));
+        v = last_lane(larger(v, dpp<0x143, 0xc>(v, v)));
+    }
     return v;
 }
 template <int G, typename R>
@@ -66,8 +85,10 @@ __device__ __forceinline__ R row_sum(R v) {
     v += dpp<0x4E>(v);
     v += dpp<0x141>(v);
     v += dpp<0x140>(v);
-    if (G > 16) v += __shfl_xor(v, 16);
-    if (G > 32) v += __shfl_xor(v, 32);
+    if constexpr (G == 64) {
+        v += dpp<0x142, 0xa>(v, (R)0);
+        v = last_lane(v + dpp<0x143, 0xc>(v, (R)0));
+    }
     return v;
 }
 
@@ -111,10 +132,10 @@ __device__ __forceinline__ bool choose(const Args& a, R (&c)[V], float floor_gap
         const int group = in_row >> a.lanes_log2;
         int rank = 0;
         for (int g = 0; g < a.groups; ++g) {
-            const R other = __shfl(value, (lane - in_row) + (g << a.lanes_log2));
+            const R other = G == 64 ? lane_value(value, g << a.lanes_log2) : __shfl(value, (lane - in_row) + (g << a.lanes_log2));
             rank += other > value || (other == value && g < group);
             if (CHECK && g != group && group < a.groups && other > -INFINITY && value > -INFINITY)
-                sure = sure && fabs((double)(other - value)) > 2 * floor_gap + 0x1p-21 * fabs((double)value);
+                sure = sure && size_of(other - value) > 2 * (R)floor_gap + (R)0x1p-21 * size_of(value);
         }
         if (rank >= a.top_groups)
 #pragma unroll
@@ -127,19 +148,32 @@ __device__ __forceinline__ bool choose(const Args& a, R (&c)[V], float floor_gap
 #pragma unroll
         for (int i = 1; i < V; ++i) best = larger(best, c[i]);
         const R top = row_max<G>(best);
-        if (CHECK && j > 0 && top > -INFINITY) sure = sure && (float)(before - top) > floor_gap + 0x1p-22f * fabsf((float)before);
+        if (CHECK && j > 0 && top > -INFINITY) sure = sure && (float)(before - top) > floor_gap + 0x1p-22f * size_of((float)before);
         if (j == a.k) break;
         before = top;
-        const u64 who = __ballot(best == top) & row_lanes;
-        const int winner = (who != 0 ? __ffsll((long long)who) : 1) - 1;
-        int slot = 0;
+        if constexpr (G == 64) {
+            u64 where[V], any = 0;
 #pragma unroll
-        for (int i = V - 1; i >= 0; --i) slot = c[i] == best ? i : slot;
-        const int expert = __shfl(first + slot, winner);
-        if (in_row == j) *mine = top > -INFINITY ? expert : -1;
-        if (lane == winner)
+            for (int i = 0; i < V; ++i) any |= where[i] = __ballot(c[i] == top);
+            const int winner = any != 0 ? __builtin_ctzll(any) : 0;
+            int slot = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = i == slot ? (R)-INFINITY : c[i];
+            for (int i = V - 1; i >= 0; --i) slot = (where[i] >> winner) & 1 ? i : slot;
+            const int expert = __builtin_amdgcn_readlane(first, winner) + slot;
+            if (in_row == j) *mine = top > -INFINITY ? expert : -1;
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = i == slot && lane == winner ? (R)-INFINITY : c[i];
+        } else {
+            const u64 who = __ballot(best == top) & row_lanes;
+            const int winner = (who != 0 ? __builtin_ctzll(who) : 0);
+            int slot = 0;
+#pragma unroll
+            for (int i = V - 1; i >= 0; --i) slot = c[i] == best ? i : slot;
+            const int expert = __shfl(first + slot, winner);
+            if (in_row == j) *mine = top > -INFINITY ? expert : -1;
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = i == slot && lane == winner ? (R)-INFINITY : c[i];
+        }
     }
     return sure;
 }
@@ -225,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             b[i] = a.bias != nullptr && i < have ? a.bias[first + i] : 0.f;
-            const float p = a.score == SCORE_SOFTMAX ? exp_of(l[i] - m) * rsum : 1.f / (1.f + exp_of(-l[i]));
+            const float p = a.score == SCORE_SOFTMAX ? exp_of(l[i] - m) * rsum : __builtin_amdgcn_rcpf(1.f + exp_of(-l[i]));
             peak = fmaxf(peak, p);
             c[i] = l[i] > -kInf ? p + b[i] : -kInf;
             bad |= !(c[i] < kInf);
@@ -286,10 +320,10 @@ hipError_t go_v(const Args& a, int v, hipStream_t stream) {
         case 1: return go<G, 1>(a, stream);
         case 2: return go<G, 2>(a, stream);
         case 4: return go<G, 4>(a, stream);
-        case 8: return go<G, 8>(a, stream);
-        case 16: return go<G, 16>(a, stream);
         default: break;
     }
+    if (v == 8) return go<G, 8>(a, stream);
+    if (v == 16) return go<G, 16>(a, stream);
     if constexpr (G == 64) return go<64, 32>(a, stream);
     return hipErrorInvalidValue;
 }
@@ -301,16 +335,17 @@ hipError_t launch_route_topk(int T, int E, int k, const void* logits, int dtype,
                              int* ids, float* weights, hipStream_t stream) {
     if (T <= 0) return hipSuccess;
     Args a{logits, row_stride, bias, ids, weights, T, E, k, dtype, score, groups, E / groups, 0, top_groups, group_top, renormalize, 0, scale};
-    // As few lanes a row as hold it with at most 16 experts a lane (with 32 only where 64 lanes do not reach otherwise):
-    // a round of the selection costs a wave the same whether it serves one row or four, so rows side by side in one wave
-    // are the cheaper way through a batch.
+    // Rows of up to 64 experts in 16 lanes with up to four each, four rows to a wave (with few experts, a wave per row leaves
+    // most lanes without work); longer ones, and such whose groups or k do not fit 16 lanes, in 64: 128 rows of 256 experts
+    // in 6 us instead of 10.  From 4096 rows on every SIMD has waves enough, and what counts is instructions a row: 16
+    // lanes with up to 16 experts each (131071 rows of 256 experts: 107 us, a wave per row 160).
+    const int most = T >= 4096 ? 16 : 4;
     int per_lane = 0, lanes = 16;
-    for (;; lanes *= 2) {
+    for (;; lanes = 64) {
         int parts = 1;
         while (parts < groups) parts *= 2;  // groups, each of lanes / parts lanes
-        const bool fits = parts <= lanes && k <= lanes;
-        const int each = fits ? (a.per + lanes / parts - 1) / (lanes / parts) : 64;
-        if (each <= 16 || lanes == 64) {
+        const int each = parts <= lanes && k <= lanes ? (a.per + lanes / parts - 1) / (lanes / parts) : 64;
+        if (each <= most || lanes == 64) {
             if (each > 32) return hipErrorInvalidValue;  // (not reached: E <= 1024 and groups <= 64)
             per_lane = 1;
             while (per_lane < each) per_lane *= 2;
@@ -321,9 +356,7 @@ hipError_t launch_route_topk(int T, int E, int k, const void* logits, int dtype,
     const int size = dtype == DTYPE_F32 ? 4 : 2;
     a.vec = a.per == (per_lane << a.lanes_log2) && (groups << a.lanes_log2) == lanes && per_lane * size % 16 == 0 &&
             row_stride * size % 16 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
-    if (lanes == 16) return go_v<16>(a, per_lane, stream);
-    if (lanes == 32) return go_v<32>(a, per_lane, stream);
-    return go_v<64>(a, per_lane, stream);
+    return lanes == 16 ? go_v<16>(a, per_lane, stream) : go_v<64>(a, per_lane, stream);
 }
 
 }  // namespace infmoe

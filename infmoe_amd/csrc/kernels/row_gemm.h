@@ -39,6 +39,22 @@ __device__ __forceinline__ v4f mma(v4u w, v4u x, v4f c, float) {
     return c;
 }
 
+// acc[j] += w[j] x for N weight operands.  (For f32 the four instructions of a piece go over the sums in turn: each depends on
+// the one before it with the same sum, and waits for it if nothing lies between.)
+template <typename T, int N>
+__device__ __forceinline__ void mma_row(v4f (&acc)[N], const v4u (&w)[N], v4u x) {
+    if constexpr (sizeof(T) == 4) {
+        const v4f b = __builtin_bit_cast(v4f, x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(v4f, w[j])[q], b[q], acc[j], 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = mma(w[j], x, acc[j], T{});
+    }
+}
+
 // 16 bytes of a row from byte k on, zeros from byte `end` on.  ALIGNED: rows start on 16-byte boundaries and `end` is a
 // multiple of 16.  Otherwise whole pieces are still one load (global memory takes 16 bytes at any address), and only the
 // piece across a row's end is put together from elements.
@@ -146,9 +162,7 @@ __device__ __forceinline__ void multiply(v4f (&acc)[S::FM][S::FN], char* lds, co
                                          const char* const (&pb)[S::kPiecesB], int end) {
     walk<T, S, ALIGNED>(lds, pa, pb, end, [&](const v4u (&wb)[S::FN], const v4u (&xa)[S::FM]) {
 #pragma unroll
-        for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-            for (int j = 0; j < S::FN; ++j) acc[i][j] = mma(wb[j], xa[i], acc[i][j], T{});
+        for (int i = 0; i < S::FM; ++i) mma_row<T, S::FN>(acc[i], wb, xa[i]);
     });
 }
 

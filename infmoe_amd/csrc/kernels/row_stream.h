@@ -40,9 +40,7 @@ __device__ __forceinline__ void stream_steps(v4f (&acc)[FM][FN], const char* con
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma(w[kk][j], x[kk][i], acc[i][j], T{});
+            for (int i = 0; i < FM; ++i) mma_row<T, FN>(acc[i], w[kk], x[kk][i]);
     };
     int s = s0;
     const int whole = min(s1, end / kStepBytes);

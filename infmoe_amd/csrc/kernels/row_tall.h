@@ -107,10 +107,7 @@ __device__ __forceinline__ void tall_multiply(v4f (&acc)[FM][4], char* lds, cons
         wb[kk][j] = *reinterpret_cast<const v4u*>(unit + at_b + place[kk] + ((j / F) * 16 * F + 4 * (j % F)) * kTallPair);
     };
     auto take_a = [&](const char* unit, int kk, int i) { xa[i] = *reinterpret_cast<const v4u*>(unit + at_a + place[kk] + i * 16 * kTallPair); };
-    auto products = [&](int kk, int i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mma(wb[kk][j], xa[i], acc[i][j], T{});
-    };
+    auto products = [&](int kk, int i) { mma_row<T, 4>(acc[i], wb[kk], xa[i]); };
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
