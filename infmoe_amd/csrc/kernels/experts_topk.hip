@@ -308,7 +308,7 @@ __global__ __launch_bounds__(kStreamThreads) void stream_kernel(Product p, FewRo
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-        stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, row_bytes);
+        stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, row_bytes, [] {});
         if (r0 > 0) __syncthreads();  // the last round's sums have been taken
         join_waves<FM, FN, NM>(lds, acc, [&](int i, int j, const v4f(&sum)[NM]) {
             const int r = r0 + i * 16 + (lane & 15), n = n0 + j * 16 + (lane >> 4) * 4;

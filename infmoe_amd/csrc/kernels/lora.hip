@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kStreamThreads) void shrink_kernel(Args p) {
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-        stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, end);
+        stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, end, [] {});
         if (again) __syncthreads();
         again = true;
         const float s = p.scale != nullptr ? p.scale[a] : 1.f;
@@ -270,6 +270,7 @@ __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) acc[i][j][q] += mine[i] == a ? sum[q] : 0.f;
                 }
+                __builtin_amdgcn_sched_barrier(0);  // one block's loads at a time: all of them at once do not fit the registers
             }
         }
 #pragma unroll
@@ -312,25 +313,53 @@ __global__ __launch_bounds__(kStreamThreads) void project_few_kernel(Args p) {
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-    stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, end);
-    join_waves<FM, FN, 1>(lds, acc, [&](int i, int j, v4f(&sum)[1]) {
-        const int t = row0 + i * 16 + (lane & 15), n = n0 + j * 16 + (lane >> 4) * 4;
-        if (t >= p.T) return;
-        const int a = p.adapter[t];
-        if (a >= 0 && a < p.L) {
+    // the adapters' part of the outputs that this lane will hold in the end (join_waves: blocks wave, wave + kStreamWaves, ...)
+    constexpr int kMine = (FM * FN + kStreamWaves - 1) / kStreamWaves;
+    v4f part[kMine];
+    auto adapters = [&] {
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+            part[c] = v4f{0.f, 0.f, 0.f, 0.f};
+            const int block = wave + c * kStreamWaves;
+            const int t = row0 + block / FN * 16 + (lane & 15), n = n0 + block % FN * 16 + (lane >> 4) * 4;
+            if (block >= FM * FN || t >= p.T) continue;
+            const int a = p.adapter[t];
+            if (a < 0 || a >= p.L) continue;
             const char *u = p.u + (size_t)t * p.u_stride, *b = p.b + ((long long)a * p.n + n) * r_end;
             for (int k = 0; k < r_end; k += 16) {
                 const v4u uk = *reinterpret_cast<const v4u*>(u + k);  // (u is padded to whole pieces)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (n + q < p.n) sum[0][q] = dot_piece<T>(uk, piece<T, B_ALIGNED>(b + q * r_end, k, r_end), sum[0][q]);
+                    if (n + q < p.n) part[c][q] = dot_piece<T>(uk, piece<T, B_ALIGNED>(b + q * r_end, k, r_end), part[c][q]);
             }
         }
+    };
+    stream_steps<T, FM, FN, ALIGNED>(acc, px, pw, steps * wave / kStreamWaves, steps * (wave + 1) / kStreamWaves, end, adapters);
+    const bool whole = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.y_stride) & (4 * sizeof(T) - 1)) == 0;
+    int c = 0;
+    join_waves<FM, FN, 1>(lds, acc, [&](int i, int j, v4f(&sum)[1]) {
+        v4f add = part[0];
+        if constexpr (kMine > 1) add = c == 0 ? part[0] : part[kMine - 1];
+        ++c;
+        const int t = row0 + i * 16 + (lane & 15), n = n0 + j * 16 + (lane >> 4) * 4;
+        if (t >= p.T) return;
         T* y = reinterpret_cast<T*>(p.y + t * p.y_stride);
+        union {
+            T e[4];
+            unsigned long long v[sizeof(T) / 2];
+        } out;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (n + q < p.n) y[n + q] = (T)sum[0][q];
+        for (int q = 0; q < 4; ++q) out.e[q] = (T)(sum[0][q] + add[q]);
+        if (whole && n + 4 <= p.n) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<unsigned long long*>(y + n) = out.v[0];
+            else *reinterpret_cast<v4u*>(y + n) = __builtin_bit_cast(v4u, out);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < p.n) y[n + q] = out.e[q];
+        }
     });
+    static_assert(kMine <= 2, "two blocks a wave at most");
 }
 
 template <typename T, int FM, int FN>
