@@ -6,6 +6,8 @@
 // rows and adds u_t B_a^T to the rows that use each: y is written once and never read.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "kernels.h"
 #include "row_gemm.h"
 #include "row_stream.h"
@@ -295,6 +297,90 @@ hipError_t go_tall(const Args& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// Rows too few for tall tiles to fill the compute units: the tiles' K is cut over `splits` workgroups, each of which leaves FP32
+// sums, and a second launch adds them and the adapters' part.  (64 rows by 10240 x 4096: 40 tiles, cut in six.  Streamed by
+// project_few_kernel the rows pass every compute unit's cache once per 64 weight rows, half of all bytes: 39 us.)
+template <typename T, int FM>
+__global__ __launch_bounds__(kTallThreads) void project_split_kernel(Args p, float* __restrict__ sums, int splits, long long sums_stride) {
+    extern __shared__ __align__(16) char lds[];
+    using W = Tall<FM, 4>;
+    constexpr int kRows = 32 * FM;
+    const int cols = (p.n + kTallCols - 1) / kTallCols;
+    const int split = blockIdx.x % splits, tile = blockIdx.x / splits;
+    const int row0 = tile / cols * kRows, n0 = tile % cols * kTallCols, count = min(kRows, p.T - row0);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+    const int end = p.d * (int)sizeof(T), pairs = (end + kTallPair - 1) / kTallPair;
+    const int k0 = (int)((long long)pairs * split / splits) * kTallPair, k1 = min((int)((long long)pairs * (split + 1) / splits) * kTallPair, end);
+    const char *pa[W::kPiecesA], *pb[4];
+#pragma unroll
+    for (int i = 0; i < W::kPiecesA; ++i) pa[i] = p.x + (row0 + min(W::row_a(i), count - 1)) * p.x_stride + k0 + W::byte_a(i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pb[i] = p.w + (long long)min(n0 + W::row_b(i), p.n - 1) * end + k0 + W::byte_b(i);
+    v4f acc[FM][4];
+    tall_multiply<T, FM, 4>(acc, lds, pa, pb, k1 - k0);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int r = (wm * FM + i) * 16 + (lane & 15);
+        if (r < count)
+            write_columns<float, 16>(sums + ((long long)split * p.T + row0 + r) * sums_stride, n0 + wn * 64 + W::column(), p.n, true,
+                                     [&](int c) { return acc[i][c >> 2][c & 3]; });
+    }
+}
+
+template <typename T, bool B_ALIGNED>
+__global__ __launch_bounds__(256) void project_join_kernel(Args p, const float* __restrict__ sums, int splits, long long sums_stride) {
+    const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (n >= p.n) return;
+    const float* from = sums + t * sums_stride + n;  // (rows are padded to four columns)
+    const long long step = p.T * sums_stride;
+    v4f sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const v4f*>(from + s * step);
+    const int a = p.adapter[t], r_end = p.r * (int)sizeof(T);
+    if (a >= 0 && a < p.L) {
+        const char *u = p.u + (size_t)t * p.u_stride, *b = p.b + ((long long)a * p.n + n) * r_end;
+        v4f part = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < r_end; k += 16) {
+            const v4u uk = *reinterpret_cast<const v4u*>(u + k);  // (u is padded to whole pieces)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < p.n) part[q] = dot_piece<T>(uk, piece<T, B_ALIGNED>(b + q * r_end, k, r_end), part[q]);
+        }
+        sum += part;
+    }
+    T* y = reinterpret_cast<T*>(p.y + t * p.y_stride);
+    if (((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.y_stride) & (4 * sizeof(T) - 1)) == 0 && n + 4 <= p.n) {
+        struct alignas(4 * sizeof(T)) Four {
+            T e[4];
+        } out;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) out.e[q] = (T)sum[q];
+        *reinterpret_cast<Four*>(y + n) = out;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (n + q < p.n) y[n + q] = (T)sum[q];
+    }
+}
+
+inline int split_height(int T) { return T <= 64 ? 2 : T <= 128 ? 4 : 8; }  // FM of the tiles
+// How many workgroups share a tile's K: what 256 compute units leave room for, at least eight pairs of steps each.
+inline int split_count(int T, int d, int n, int size) {
+    const long long tiles = (long long)((T + 32 * split_height(T) - 1) / (32 * split_height(T))) * ((n + kTallCols - 1) / kTallCols);
+    const long long most = std::min<long long>(256 / tiles, (long long)d * size / (8 * kTallPair));
+    return (int)std::max<long long>(1, most);
+}
+
+template <typename T, int FM>
+hipError_t go_split(const Args& p, float* sums, int splits, bool b_aligned, hipStream_t stream) {
+    const long long tiles = (long long)((p.T + 32 * FM - 1) / (32 * FM)) * ((p.n + kTallCols - 1) / kTallCols), stride = (p.n + 3) / 4 * 4;
+    if (const hipError_t err = allow_lds_once<project_split_kernel<T, FM>>(kTallLds); err != hipSuccess) return err;
+    project_split_kernel<T, FM><<<(int)(tiles * splits), kTallThreads, kTallLds, stream>>>(p, sums, splits, stride);
+    const dim3 grid((p.n + 1023) / 1024, p.T);
+    if (b_aligned) project_join_kernel<T, true><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
+    else project_join_kernel<T, false><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
+    return hipGetLastError();
+}
+
 // Few rows: W streamed once through the registers, 16 * FN of its rows per workgroup; the adapters' part of an output is added
 // by the lane that holds the joined sum.
 template <typename T, int FM, int FN, bool ALIGNED, bool B_ALIGNED>
@@ -388,7 +474,7 @@ hipError_t go(const Args& p, hipStream_t stream) {
 }
 
 template <typename T>
-hipError_t run(const Args& p, hipStream_t stream) {
+hipError_t run(const Args& p, float* sums, hipStream_t stream) {
     using S = Shape<1, 4, 4, 2>;
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | p.x_stride | p.d * sizeof(T)) & 15) == 0;
     const bool a_aligned = aligned && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
@@ -412,6 +498,13 @@ hipError_t run(const Args& p, hipStream_t stream) {
     const long long columns = (p.n + kTallCols - 1) / kTallCols;
     if (aligned && (p.T + 255) / 256 * columns >= 200) return b_aligned ? go_tall<T, 8, true>(p, stream) : go_tall<T, 8, false>(p, stream);
     if (aligned && (p.T + 127) / 128 * columns >= 100) return b_aligned ? go_tall<T, 4, true>(p, stream) : go_tall<T, 4, false>(p, stream);
+    if (aligned && p.T > 16) {
+        const int splits = split_count(p.T, p.d, p.n, sizeof(T));
+        if (splits > 1) {
+            if (split_height(p.T) == 2) return go_split<T, 2>(p, sums, splits, b_aligned, stream);
+            return split_height(p.T) == 4 ? go_split<T, 4>(p, sums, splits, b_aligned, stream) : go_split<T, 8>(p, sums, splits, b_aligned, stream);
+        }
+    }
     // Streams of up to 64 rows: W passes once per 64 rows.  The rows come through the caches, FM / FN of the weights' bytes,
     // so as many weight rows per workgroup as leave at least 128 workgroups (64 rows by 10240 x 4096: 16 weight rows 64 us,
     // 64 of them 26).  With more rows, as long as tiles of 64 x 128 would leave compute units without work.
@@ -430,8 +523,11 @@ inline int u_stride_bytes(int r, int size) { return (r * size + 15) / 16 * 16; }
 
 }  // namespace
 
-size_t lora_project_workspace_bytes(int T, int, int, int r, int dtype) {
-    return ((size_t)T * u_stride_bytes(r, dtype == DTYPE_F32 ? 4 : 2) + 255) & ~(size_t)255;
+inline size_t u_bytes(int T, int r, int size) { return ((size_t)T * u_stride_bytes(r, size) + 255) & ~(size_t)255; }
+
+size_t lora_project_workspace_bytes(int T, int d, int n, int r, int dtype) {
+    const int size = dtype == DTYPE_F32 ? 4 : 2, splits = T > 16 ? split_count(T, d, n, size) : 1;
+    return u_bytes(T, r, size) + (splits > 1 ? (size_t)splits * T * ((n + 3) / 4 * 4) * 4 : 0);
 }
 
 hipError_t launch_lora_project(int T, int d, int n, int r, int L, int dtype, const void* x, long long x_stride, const void* w, const void* a,
@@ -442,9 +538,10 @@ hipError_t launch_lora_project(int T, int d, int n, int r, int L, int dtype, con
     auto in = [](const void* p) { return static_cast<const char*>(p); };
     const Args p{in(x), in(w), in(a), in(b), static_cast<char*>(workspace), static_cast<char*>(y), adapter, scale, x_stride * size, y_stride * size,
                  T, d, n, r, L, u_stride_bytes(r, size)};
-    if (dtype == DTYPE_F32) return run<float>(p, stream);
-    if (dtype == DTYPE_F16) return run<_Float16>(p, stream);
-    return run<__bf16>(p, stream);
+    float* sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + u_bytes(T, r, size));
+    if (dtype == DTYPE_F32) return run<float>(p, sums, stream);
+    if (dtype == DTYPE_F16) return run<_Float16>(p, sums, stream);
+    return run<__bf16>(p, sums, stream);
 }
 
 }  // namespace infmoe

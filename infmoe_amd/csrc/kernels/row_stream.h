@@ -24,7 +24,9 @@ __device__ __forceinline__ void stream_steps(v4f (&acc)[FM][FN], const char* con
     constexpr int DEPTH = FM + FN <= 2 ? 4 : FM + FN <= 4 ? 3 : 2;
     const int lane_at = (threadIdx.x & 63) >> 4 << 4, whole = end / kStepBytes;
     v4u w[DEPTH][2][FN], x[DEPTH][2][FM];
-    auto ask = [&](int d, int s) {
+    const int n = s1 - s0, turn = n > 0 ? (int)(blockIdx.x / kXcdCount * 2) % n : 0;
+    auto ask = [&](int d, int q) {
+        const int s = s0 + (q + turn >= n ? q + turn - n : q + turn);
         const int k = s * kStepBytes + lane_at;
         if (s < whole) {
             // (the two halves of a line one after the other; kept in the caches for just that, where a hint that the
@@ -49,19 +51,19 @@ __device__ __forceinline__ void stream_steps(v4f (&acc)[FM][FN], const char* con
     };
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
-        if (s0 + d < s1) ask(d, s0 + d);
+        if (d < n) ask(d, d);
     between();
 #pragma unroll 1
-    for (int s = s0; s < s1; s += DEPTH) {
+    for (int q = 0; q < n; q += DEPTH) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            if (s + d < s1) {
+            if (q + d < n) {
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                     for (int i = 0; i < FM; ++i) mma_row<T, FN>(acc[i], w[d][kk], x[d][kk][i]);
             }
-            if (s + d + DEPTH < s1) ask(d, s + d + DEPTH);
+            if (q + d + DEPTH < n) ask(d, q + d + DEPTH);
         }
     }
 }
