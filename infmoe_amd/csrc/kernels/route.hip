@@ -109,38 +109,107 @@ __device__ __forceinline__ float exp_of(float x) { return __expf(x); }
 // quotient's, all in all under 16 u p_max.  The sum with the bias is rounded once: u |p + bias|.  Two such errors, either way.
 constexpr float kScoreError = 0x1p-19f;  // 32 u
 
-// The choice of the k best of one row per G lanes.  R: float, or double for the rows that FP32 cannot order.  Lane j of the
-// row gets the j-th expert in *mine (-1: nothing left to choose).  Returns whether the row is ordered for certain
-// (CHECK; the same answer in all of a row's lanes).
+// The experts of all but the top_groups best groups masked.  R: float, or double for the rows that FP32 cannot order.  Returns
+// whether the choice of groups is certain (CHECK).
 template <typename R, bool CHECK, int G, int V>
-__device__ __forceinline__ bool choose(const Args& a, R (&c)[V], float floor_gap, int in_row, u64 row_lanes, int first, int* mine) {
+__device__ __forceinline__ bool keep_groups(const Args& a, R (&c)[V], float floor_gap, int in_row) {
     const int lane = threadIdx.x & 63;
     bool sure = true;
-    if (a.groups > 1) {
-        R one = -INFINITY, two = -INFINITY;  // the two largest of the lane's, then of its group's lanes
+    R one = -INFINITY, two = -INFINITY;  // the two largest of the lane's, then of its group's lanes
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            two = larger(two, one < c[i] ? one : c[i]);
-            one = larger(one, c[i]);
-        }
-        for (int step = 1; step < (1 << a.lanes_log2); step <<= 1) {
-            const R o1 = __shfl_xor(one, step), o2 = __shfl_xor(two, step);
-            two = larger(larger(two, o2), one < o1 ? one : o1);
-            one = larger(one, o1);
-        }
-        const R value = a.group_top == 2 ? one + two : one;
-        const int group = in_row >> a.lanes_log2;
-        int rank = 0;
-        for (int g = 0; g < a.groups; ++g) {
-            const R other = G == 64 ? lane_value(value, g << a.lanes_log2) : __shfl(value, (lane - in_row) + (g << a.lanes_log2));
-            rank += other > value || (other == value && g < group);
-            if (CHECK && g != group && group < a.groups && other > -INFINITY && value > -INFINITY)
-                sure = sure && size_of(other - value) > 2 * (R)floor_gap + (R)0x1p-21 * size_of(value);
-        }
-        if (rank >= a.top_groups)
-#pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = -INFINITY;
+    for (int i = 0; i < V; ++i) {
+        two = larger(two, one < c[i] ? one : c[i]);
+        one = larger(one, c[i]);
     }
+    for (int step = 1; step < (1 << a.lanes_log2); step <<= 1) {
+        const R o1 = __shfl_xor(one, step), o2 = __shfl_xor(two, step);
+        two = larger(larger(two, o2), one < o1 ? one : o1);
+        one = larger(one, o1);
+    }
+    const R value = a.group_top == 2 ? one + two : one;
+    const int group = in_row >> a.lanes_log2;
+    int rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+        const R other = G == 64 ? lane_value(value, g << a.lanes_log2) : __shfl(value, (lane - in_row) + (g << a.lanes_log2));
+        rank += other > value || (other == value && g < group);
+        if (CHECK && g != group && group < a.groups && other > -INFINITY && value > -INFINITY)
+            sure = sure && size_of(other - value) > 2 * (R)floor_gap + (R)0x1p-21 * size_of(value);
+    }
+    if (rank >= a.top_groups)
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = -INFINITY;
+    return sure;
+}
+
+// Whether two neighbours of the ranking are far enough apart for FP32.
+__device__ __forceinline__ bool apart(float larger_one, float smaller, float floor_gap) {
+    return !(smaller > -kInf) || larger_one - smaller > floor_gap + 0x1p-22f * size_of(larger_one);
+}
+
+// The k best of rows of 16 lanes from a short list, when one can be had: t, the (k + 1)-th largest among the two best of every
+// lane, is reached by k + 1 experts at least and, unless many are equal or few lanes take part, by no more than 16.  Those go
+// through LDS to a lane each, in order of their indices; there every lane counts who is before it, and the counts are the
+// ranking.  (k + 1 rounds of choose_rounds instead: 1580 vector instructions a wave for 131071 rows of 256, 107 us.)
+// Returns false, for all rows of the wave, where a list is too long.
+template <bool CHECK, int V>
+__device__ __forceinline__ bool choose_listed(const Args& a, const float (&c)[V], float floor_gap, int in_row, int first, float2* list, int* mine, bool* sure) {
+    float one = -kInf, two = -kInf;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        two = larger(two, one < c[i] ? one : c[i]);
+        one = larger(one, c[i]);
+    }
+    int before_one = 0, before_two = one > two;
+    auto against = [&](float o1, float o2) {
+        before_one += o1 > one, before_one += o2 > one;
+        before_two += o1 > two, before_two += o2 > two;
+    };
+#define INFMOE_EACH_TURN(X) X(1) X(2) X(3) X(4) X(5) X(6) X(7) X(8) X(9) X(10) X(11) X(12) X(13) X(14) X(15)
+#define INFMOE_TURN(r) against(dpp<0x120 + r>(one), dpp<0x120 + r>(two));  // of the lane r before, around the 16
+    INFMOE_EACH_TURN(INFMOE_TURN)
+#undef INFMOE_TURN
+    float t = before_two <= a.k ? two : before_one <= a.k ? one : kInf;
+    t = -row_max<16>(-t);                     // the smallest of those that at most k are before
+    t = larger(t, -3.4028235e38f);            // (a masked expert is never listed)
+    int here = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) here += c[i] >= t;
+    int to = here;  // listed in this lane and those before it
+#define INFMOE_SCAN(ctrl) to += __builtin_amdgcn_update_dpp(0, to, ctrl, 0xf, 0xf, false);
+    INFMOE_SCAN(0x111) INFMOE_SCAN(0x112) INFMOE_SCAN(0x114) INFMOE_SCAN(0x118)
+#undef INFMOE_SCAN
+    if (__ballot(to > 16) != 0) return false;
+    float2* row = list + ((threadIdx.x & 63) >> 4) * 16;  // (one wave's LDS operations are done in order)
+    row[in_row] = float2{-kInf, __int_as_float(-1)};
+    int at = to - here;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (c[i] >= t) row[at++] = float2{c[i], __int_as_float(first + i)};
+    const float2 entry = row[in_row];
+    int rank = 0;
+    // an equal one counts as before where its lane, and so its index, is lower
+#define INFMOE_TURN(r)                                              \
+    {                                                               \
+        const float other = dpp<0x120 + r>(entry.x);                \
+        rank += other > entry.x || (other == entry.x && in_row >= r); \
+    }
+    INFMOE_EACH_TURN(INFMOE_TURN)
+#undef INFMOE_TURN
+#undef INFMOE_EACH_TURN
+    row[rank] = entry;
+    const float2 mine_now = row[in_row];
+    *mine = in_row < a.k ? __float_as_int(mine_now.y) : -1;
+    const float next = dpp<0x101>(mine_now.x, -kInf);  // of the lane behind; read by all lanes, a lane that is left out gives nothing
+    if (CHECK) *sure = in_row >= a.k || apart(mine_now.x, next, floor_gap);
+    return true;
+}
+
+// The k best of one row per G lanes, one after the other.  Lane j of the row gets the j-th expert in *mine (-1: nothing left
+// to choose).  Returns whether the row is ordered for certain (CHECK; the same answer in all of a row's lanes).
+template <typename R, bool CHECK, int G, int V>
+__device__ __forceinline__ bool choose_rounds(const Args& a, R (&c)[V], float floor_gap, int in_row, u64 row_lanes, int first, int* mine) {
+    const int lane = threadIdx.x & 63;
+    bool sure = true;
     R before = INFINITY;
     const int rounds = CHECK ? a.k + 1 : a.k;  // the border to the first expert left out counts too
     for (int j = 0; j < rounds; ++j) {
@@ -148,7 +217,7 @@ __device__ __forceinline__ bool choose(const Args& a, R (&c)[V], float floor_gap
 #pragma unroll
         for (int i = 1; i < V; ++i) best = larger(best, c[i]);
         const R top = row_max<G>(best);
-        if (CHECK && j > 0 && top > -INFINITY) sure = sure && (float)(before - top) > floor_gap + 0x1p-22f * size_of((float)before);
+        if (CHECK && j > 0) sure = sure && apart((float)before, (float)top, floor_gap);
         if (j == a.k) break;
         before = top;
         if constexpr (G == 64) {
@@ -178,8 +247,22 @@ __device__ __forceinline__ bool choose(const Args& a, R (&c)[V], float floor_gap
     return sure;
 }
 
+// Groups, then the k best.
+template <typename R, bool CHECK, int G, int V>
+__device__ __forceinline__ bool choose(const Args& a, R (&c)[V], float floor_gap, int in_row, u64 row_lanes, int first, float2* list, int* mine) {
+    bool sure = true;
+    if (a.groups > 1) sure = keep_groups<R, CHECK, G, V>(a, c, floor_gap, in_row);
+    if constexpr (G == 16 && V >= 8 && sizeof(R) == 4) {
+        bool ordered = true;
+        if (a.k <= 15 && choose_listed<CHECK, V>(a, c, floor_gap, in_row, first, list, mine, &ordered)) return sure && ordered;
+    }
+    return choose_rounds<R, CHECK, G, V>(a, c, floor_gap, in_row, row_lanes, first, mine) && sure;
+}
+
 template <int G, int V>
 __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
+    __shared__ float2 s_list[kThreads];  // choose_listed: 64 entries a wave
+    float2* list = s_list + (threadIdx.x & ~63);
     const int lane = threadIdx.x & 63, in_row = lane & (G - 1);
     const u64 row_lanes = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1)) << (lane - in_row);
     const long long row = ((long long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * (64 / G) + lane / G;
@@ -228,8 +311,9 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
     }
 
     bool bad = false;  // no order: a NaN, or a softmax over an infinite logit
+    const float finite = a.score == SCORE_SOFTMAX ? 3.4028235e38f : kInf;
 #pragma unroll
-    for (int i = 0; i < V; ++i) bad |= l[i] != l[i] || (a.score == SCORE_SOFTMAX && l[i] == kInf);
+    for (int i = 0; i < V; ++i) bad |= !(l[i] <= finite);
 
     const bool scored = a.bias != nullptr || a.group_top == 2;
     float m = 0.f, sum = 1.f;
@@ -252,34 +336,53 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
         float c[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) c[i] = l[i];
-        choose<float, false, G, V>(a, c, 0.f, in_row, row_lanes, first, &mine);
+        choose<float, false, G, V>(a, c, 0.f, in_row, row_lanes, first, list, &mine);
     } else {
         float c[V], b[V], peak = 0x1p-10f;
-        const float rsum = 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[i] = 0.f;
+        if (a.bias != nullptr) {
+            if (a.vec) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) b[i] = a.bias[first + i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) b[i] = i < have ? a.bias[first + i] : 0.f;
+            }
+        }
+        if (a.score == SCORE_SOFTMAX) {
+            const float rsum = 1.f / sum;
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = exp_of(l[i] - m) * rsum;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = __builtin_amdgcn_rcpf(1.f + exp_of(-l[i]));
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            b[i] = a.bias != nullptr && i < have ? a.bias[first + i] : 0.f;
-            const float p = a.score == SCORE_SOFTMAX ? exp_of(l[i] - m) * rsum : __builtin_amdgcn_rcpf(1.f + exp_of(-l[i]));
-            peak = fmaxf(peak, p);
-            c[i] = l[i] > -kInf ? p + b[i] : -kInf;
+            peak = fmaxf(peak, c[i]);
+            c[i] = l[i] > -kInf ? c[i] + b[i] : -kInf;
             bad |= !(c[i] < kInf);
         }
         peak = row_max<G>(peak);
-        bool sure = choose<float, true, G, V>(a, c, kScoreError * peak, in_row, row_lanes, first, &mine);
+        bool sure = choose<float, true, G, V>(a, c, kScoreError * peak, in_row, row_lanes, first, list, &mine);
         if (__ballot(!sure && !bad) != 0) {  // some row of this wave: all of its rows again, in 64 bits
-            double d[V], total = 0.0;
+            double d[V];
             if (a.score == SCORE_SOFTMAX) {
+                double total = 0.0;
 #pragma unroll
-                for (int i = 0; i < V; ++i) total += exp((double)l[i] - m);
+                for (int i = 0; i < V; ++i) total += d[i] = exp((double)l[i] - m);
                 total = row_sum<G>(total);
+#pragma unroll
+                for (int i = 0; i < V; ++i) d[i] /= total;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) d[i] = 1.0 / (1.0 + exp(-(double)l[i]));
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double p = a.score == SCORE_SOFTMAX ? exp((double)l[i] - m) / total : 1.0 / (1.0 + exp(-(double)l[i]));
-                d[i] = l[i] > -kInf ? p + (double)b[i] : -INFINITY;
-            }
+            for (int i = 0; i < V; ++i) d[i] = l[i] > -kInf ? d[i] + (double)b[i] : -INFINITY;
             mine = -1;
-            choose<double, false, G, V>(a, d, 0.f, in_row, row_lanes, first, &mine);
+            choose<double, false, G, V>(a, d, 0.f, in_row, row_lanes, first, list, &mine);
         }
     }
     const bool nan_row = (__ballot(bad) & row_lanes) != 0;

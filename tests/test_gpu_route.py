@@ -115,6 +115,32 @@ def test_masked_and_unordered_rows(lib, torch_cuda, score, scored, groups, top_g
     assert np.isnan(want[1][11]).all()
 
 
+@pytest.mark.parametrize("E,k,groups,top_groups,group_top", [
+    (256, 8, 8, 4, 2), (256, 15, 1, 1, 1), (200, 6, 1, 1, 1), (128, 8, 4, 1, 2), (96, 2, 3, 2, 1), (250, 16, 1, 1, 1), (72, 10, 8, 2, 1)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_large_batches(lib, torch_cuda, E, k, groups, top_groups, group_top, score):
+    """Batches long enough for several rows of many experts per wave, with everything a row can bring on the way: equal scores
+    (more of them than a short list holds), masked experts, rows without order, scores closer than FP32 orders."""
+    torch = torch_cuda
+    from infmoe_amd import ops
+    rng = np.random.default_rng(E + k)
+    T = 4101
+    x = (2.0 * rng.standard_normal((T, E))).astype(np.float32)
+    x[1::7] = np.round(x[1::7])                       # many equal
+    x[2] = 0.5                                        # all equal
+    x[3, 5:] = -np.inf
+    x[4] = -np.inf
+    x[5, 1] = np.nan
+    x[6, 2] = np.inf
+    x[9::11][rng.random((len(x[9::11]), E)) < 0.5] = -np.inf
+    x[4100, :E // 2] = x[4100, E // 2:E // 2 * 2]
+    near = (10.0 ** rng.uniform(-9, -6, E) * rng.choice([-1, 1], E)).astype(np.float32)
+    for dtype, bias in (("float32", None), ("float32", near), ("bfloat16", near), ("float16", None)):
+        t, exact = tensors(torch, x, dtype)
+        kw = dict(score=score, groups=groups, top_groups=top_groups, group_top=group_top)
+        check(ops.route_topk(t, k, bias=None if bias is None else torch.from_numpy(bias).cuda(), **kw), O.route_topk(exact, k, bias=bias, **kw))
+
+
 def test_strided_rows_offsets_and_given_outputs(lib, torch_cuda):
     torch = torch_cuda
     from infmoe_amd import ops
