@@ -238,7 +238,7 @@ hipError_t launch_experts_topk(int T, int k, int E, int d, int h, int ffn, int d
 
 // ---- a projection with a low-rank adapter per row (no counterpart in the reference)
 // w [n][d], a [L][r][d], b [L][n][r], r <= kLoraMaxRank; a row whose adapter is outside [0, L) has none; scale null: 1.
-constexpr int kLoraMaxRank = 256, kRowsMaxLength = 1 << 24;  // (a row's bytes fit 31 bits)
+constexpr int kLoraMaxRank = 256, kRowsMaxLength = 1 << 23;  // (a row's bytes fit 31 bits, its blocks of 256 a grid's 16)
 size_t lora_project_workspace_bytes(int T, int d, int n, int r, int dtype);
 hipError_t launch_lora_project(int T, int d, int n, int r, int L, int dtype, const void* x, long long x_stride, const void* w, const void* a,
                                const void* b, const int* adapter, const float* scale, void* y, long long y_stride, void* workspace,

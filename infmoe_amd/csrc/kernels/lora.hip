@@ -1,9 +1,12 @@
 // A projection shared by all rows of a batch with a low-rank adapter per row, for gfx950:
 //   y_t = W x_t + scale_a * B_a (A_a x_t),  a = adapter[t].
 //
-// Two launches: `shrink` forms u_t = scale_a * A_a x_t ([T][r], in the operands' type, as the second product takes it);
-// `project` computes W x_t and, before its tile leaves the registers, goes over the adapters that occur among the tile's
-// rows and adds u_t B_a^T to the rows that use each: y is written once and never read.
+// The first launch forms u_t = scale_a * A_a x_t ([T][r], in the operands' type, as the second product takes it), the next
+// computes W x_t and adds u_t B_a^T before its results leave the registers, so that y is written once and never read:
+//   up to 16 rows, odd strides      W streamed through the registers (project_few_kernel)
+//   many rows                       tall tiles, which go over the adapters that occur among their rows (project_tall_kernel)
+//   between the two                 tall tiles with K cut over workgroups, joined by a third launch (project_split_kernel)
+//   many rows of odd strides        tiles of 64 x 128 (project_kernel)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -40,6 +40,30 @@ def test_experts_at_long_rows(lib, torch_cuda, dtype, T):
     assert_within(call(ops, c), *O.experts_topk(**c["exact"]), what=dtype)
 
 
+@pytest.mark.parametrize("dtype,ffn", [("bfloat16", "gated_silu"), ("float16", "relu"), ("float32", "gated_gelu")])
+def test_experts_on_tall_tiles(lib, torch_cuda, dtype, ffn):
+    """Enough rows and columns for tiles of up to 256 x 256: experts with no row, one row, a few, and several tiles; row lengths
+    that are no whole number of steps.  A sample of the tokens against the oracle, the others by a second call in which the
+    tokens stand in another order."""
+    torch = torch_cuda
+    from infmoe_amd import ops
+    T, k, E, d, h = 1280, 3, 16, 2056, 2072
+    rng = np.random.default_rng(12)
+    c = draw_experts(torch, rng, T, k, E, d, h, ffn, dtype)
+    odds = np.array([0, 0.0002, 0.01, 0.02, 0.05, 0.05, 0.06, 0.07, 0.08, 0.08, 0.08, 0.09, 0.1, 0.1, 0.1, 0.1])
+    ids = rng.choice(E, size=(T, k), p=odds / odds.sum()).astype(np.int32)
+    ids[17] = [1, 1, 15]
+    ids[18] = -1
+    c["ids"].copy_(torch.from_numpy(ids))
+    y = call(ops, c)
+    some = np.concatenate([[17, 18], rng.choice(T, 40, replace=False)])
+    exact = dict(c["exact"], x=c["exact"]["x"][some], ids=ids[some], weights=c["exact"]["weights"][some])
+    assert_within(y[torch.from_numpy(some).cuda()], *O.experts_topk(**exact), what=f"{dtype} {ffn}")
+    order = torch.from_numpy(rng.permutation(T)).cuda()
+    again = ops.experts_topk(c["x"][order], c["ids"][order], c["weights"][order], c["wi"], c["wo"], c["wi_1"], ffn=ffn)
+    assert torch.equal(again, y[order])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,E,k", [(6, 5, 3), (200, 6, 2), (40, 3, 4)])
 def test_ids_that_are_no_expert_and_ids_twice(lib, torch_cuda, dtype, T, E, k):

@@ -39,6 +39,16 @@ def test_lora_at_long_rows(lib, torch_cuda, dtype, T):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,d,n,r,L", [(3000, 64, 4500, 16, 5), (1500, 72, 2300, 12, 3), (100, 2048, 520, 16, 5), (30, 4096, 260, 20, 9), (240, 1032, 776, 8, 4)])
+@pytest.mark.parametrize("order", ["any", "requests"])
+def test_lora_on_tall_tiles(lib, torch_cuda, dtype, T, d, n, r, L, order):
+    """Tiles of 256 and of 128 rows, and tiles whose K is cut over workgroups (two, four and eight blocks of rows)."""
+    from infmoe_amd import ops
+    c = draw_lora(torch_cuda, np.random.default_rng(T + n), T, d, n, r, L, dtype, order)
+    assert_within(call(ops, c), *O.lora_project(**c["exact"]), what=dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [3, 20, 150])
 def test_one_adapter_cannot_reach_the_rows_of_another(lib, torch_cuda, dtype, T):
     torch = torch_cuda
@@ -50,9 +60,27 @@ def test_one_adapter_cannot_reach_the_rows_of_another(lib, torch_cuda, dtype, T)
     c["b"][2, 7, 1] = float("inf")
     c["b"][3] = float("nan")
     y = call(ops, c)
-    fine = (c["adapter"] <= 0).nonzero()[:, 0]
+    fine = (c["adapter"] <= 0).nonzero()[:, 0]  # (none, or adapter 0)
     assert torch.equal(y[fine], clean[fine])
     assert all(not y[t].isfinite().all() for t in range(T) if int(c["adapter"][t]) > 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,n", [(3000, 4500), (1500, 2300), (90, 264)])
+def test_one_adapter_cannot_reach_the_rows_of_another_on_tall_tiles(lib, torch_cuda, dtype, T, n):
+    torch = torch_cuda
+    from infmoe_amd import ops
+    d = 2048 if T < 100 else 64
+    c = draw_lora(torch, np.random.default_rng(2), T, d, n, 8, 4, dtype, "any")
+    c["adapter"][:] = torch.arange(T, dtype=torch.int32, device="cuda") % 5 - 1
+    clean = call(ops, c)
+    c["b"][2, 7, 1] = float("inf")
+    c["b"][3] = float("nan")
+    c["x"][0] = float("nan")  # (a row without an adapter)
+    y = call(ops, c)
+    fine = ((c["adapter"] >= 0) & (c["adapter"] <= 1)).nonzero()[:, 0]
+    assert torch.equal(y[fine], clean[fine])
+    assert y[0].isnan().all() and y[3::5].isfinite().all(dim=1).sum() == 0 and y[4::5].isnan().all()
 
 
 def test_no_adapter_anywhere_no_scale_and_padding_rows(lib, torch_cuda):
