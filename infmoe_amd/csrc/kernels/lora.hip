@@ -334,14 +334,17 @@ template <typename T, bool B_ALIGNED>
 __global__ __launch_bounds__(256) void project_join_kernel(Args p, const float* __restrict__ sums, int splits, long long sums_stride) {
     const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
     if (n >= p.n) return;
+    const int a = p.adapter[t];
     const float* from = sums + t * sums_stride + n;  // (rows are padded to four columns)
     const long long step = p.T * sums_stride;
     v4f sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const v4f*>(from + s * step);
-    const int a = p.adapter[t], r_end = p.r * (int)sizeof(T);
+    const int r_end = p.r * (int)sizeof(T);
     if (a >= 0 && a < p.L) {
         const char *u = p.u + (size_t)t * p.u_stride, *b = p.b + ((long long)a * p.n + n) * r_end;
         v4f part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
         for (int k = 0; k < r_end; k += 16) {
             const v4u uk = *reinterpret_cast<const v4u*>(u + k);  // (u is padded to whole pieces)
 #pragma unroll

@@ -56,8 +56,8 @@ __device__ __forceinline__ void mma_row(v4f (&acc)[N], const v4u (&w)[N], v4u x)
 }
 
 // 16 bytes of a row from byte k on, zeros from byte `end` on.  ALIGNED: rows start on 16-byte boundaries and `end` is a
-// multiple of 16.  Otherwise whole pieces are still one load (global memory takes 16 bytes at any address), and only the
-// piece across a row's end is put together from elements.
+// multiple of 16.  Otherwise whole pieces are still one load (global memory takes 16 bytes at any address); the piece across a
+// row's end is the row's last 16 bytes, shifted, and only of rows shorter than that put together from elements.
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ v4u whole_piece(const char* at) {
     if constexpr (ALIGNED) return *reinterpret_cast<const v4u*>(at);
@@ -72,6 +72,18 @@ __device__ __forceinline__ v4u piece(const char* row, int k, int end) {
         return k < end ? v : v4u{0, 0, 0, 0};
     } else {
         if (k + 16 <= end) return whole_piece<T, false>(row + k);
+        if (k >= end) return v4u{0, 0, 0, 0};
+        if (end >= 16) {
+            union {
+                v4u v;
+                unsigned long long half[2];
+            } last{whole_piece<T, false>(row + end - 16)};
+            const int by = 8 * (k + 16 - end);  // bits; 8 to 120
+            const unsigned long long low = last.half[0], high = last.half[1];
+            last.half[0] = by >= 64 ? high >> (by - 64) : low >> by | high << (64 - by);
+            last.half[1] = by >= 64 ? 0 : high >> by;
+            return last.v;
+        }
         union {
             T e[16 / sizeof(T)];
             v4u v;
