@@ -330,42 +330,24 @@ __global__ __launch_bounds__(kTallThreads) void project_split_kernel(Args p, flo
     }
 }
 
+// (A thread per column: the lanes of a wave read rows of B_a that lie side by side.)
 template <typename T, bool B_ALIGNED>
 __global__ __launch_bounds__(256) void project_join_kernel(Args p, const float* __restrict__ sums, int splits, long long sums_stride) {
-    const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const int t = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
     if (n >= p.n) return;
-    const int a = p.adapter[t];
-    const float* from = sums + t * sums_stride + n;  // (rows are padded to four columns)
+    const int a = p.adapter[t], r_end = p.r * (int)sizeof(T);
+    const float* from = sums + t * sums_stride + n;
     const long long step = p.T * sums_stride;
-    v4f sum = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f, part = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const v4f*>(from + s * step);
-    const int r_end = p.r * (int)sizeof(T);
+    for (int s = 0; s < splits; ++s) sum += from[s * step];
     if (a >= 0 && a < p.L) {
         const char *u = p.u + (size_t)t * p.u_stride, *b = p.b + ((long long)a * p.n + n) * r_end;
-        v4f part = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
-        for (int k = 0; k < r_end; k += 16) {
-            const v4u uk = *reinterpret_cast<const v4u*>(u + k);  // (u is padded to whole pieces)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (n + q < p.n) part[q] = dot_piece<T>(uk, piece<T, B_ALIGNED>(b + q * r_end, k, r_end), part[q]);
-        }
-        sum += part;
+        for (int k = 0; k < r_end; k += 16)  // (u is padded to whole pieces)
+            part = dot_piece<T>(*reinterpret_cast<const v4u*>(u + k), piece<T, B_ALIGNED>(b, k, r_end), part);
     }
-    T* y = reinterpret_cast<T*>(p.y + t * p.y_stride);
-    if (((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.y_stride) & (4 * sizeof(T) - 1)) == 0 && n + 4 <= p.n) {
-        struct alignas(4 * sizeof(T)) Four {
-            T e[4];
-        } out;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) out.e[q] = (T)sum[q];
-        *reinterpret_cast<Four*>(y + n) = out;
-    } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (n + q < p.n) y[n + q] = (T)sum[q];
-    }
+    reinterpret_cast<T*>(p.y + t * p.y_stride)[n] = (T)(sum + part);
 }
 
 inline int split_height(int T) { return T <= 64 ? 2 : T <= 128 ? 4 : 8; }  // FM of the tiles
@@ -381,7 +363,7 @@ hipError_t go_split(const Args& p, float* sums, int splits, bool b_aligned, hipS
     const long long tiles = (long long)((p.T + 32 * FM - 1) / (32 * FM)) * ((p.n + kTallCols - 1) / kTallCols), stride = (p.n + 3) / 4 * 4;
     if (const hipError_t err = allow_lds_once<project_split_kernel<T, FM>>(kTallLds); err != hipSuccess) return err;
     project_split_kernel<T, FM><<<(int)(tiles * splits), kTallThreads, kTallLds, stream>>>(p, sums, splits, stride);
-    const dim3 grid((p.n + 1023) / 1024, p.T);
+    const dim3 grid((p.n + 255) / 256, p.T);
     if (b_aligned) project_join_kernel<T, true><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
     else project_join_kernel<T, false><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
     return hipGetLastError();
