@@ -11,7 +11,8 @@
 // second product's operand has.  The rows that combine adds stay in FP32: one more rounding there would be seen in y.
 //
 // Three forms of the products, by rows per expert on average (slots / E):
-//   up to 16   the weights streamed once through the registers, tiles of 16 rows (up to 4 on average) or 32 (stream_kernel).
+//   up to 8 (16 where there are no tall tiles)
+//              the weights streamed once through the registers, tiles of 16 rows (up to 4 on average) or 32 (stream_kernel).
 //              At 4 a tile of 64 x 128 through LDS took 1.05 ms where the stream takes 0.85 (32 experts of 4096 x 10240);
 //   more       tall tiles where there are enough for the compute units (tall_kernel): 4096 tokens over the same experts take
 //              4.9 ms in tiles of 64 x 128 and 2.4 in tall ones; with 96 tall tiles for 256 compute units, f32, 3009 rows
@@ -469,14 +470,15 @@ hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long lon
                const Carve& c, hipStream_t stream) {
     using S = Shape<1, 4, 4, 2>;
     const int slots = Tn * k, blocks = (slots + kPlanBlock - 1) / kPlanBlock;
-    // few rows per expert: tiles of 16 or 32 rows, weights streamed
-    const int few_blocks = slots <= 4 * E ? 1 : slots <= 16 * E ? 2 : 0;
-    const bool mini = few_blocks > 0 && slots <= kMiniSlots;
     auto on16 = [](const void* p, long long stride) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (long long)sizeof(T))) & 15) == 0; };
     const bool in_ok = d * sizeof(T) % 16 == 0 && on16(x, x_stride) && on16(wi, wi_stride) && on16(wi_1, 0);
     const bool out_ok = h * sizeof(T) % 16 == 0 && on16(wo, wo_stride);
-    const bool tall = few_blocks == 0 && in_ok && out_ok &&
-                      (slots / kTallRows + std::min(E, slots) / 2) * (long long)((std::min(d, h) + kTallCols - 1) / kTallCols) >= 200;
+    // tall tiles, if about as many as compute units can be expected (f32, whose small tiles are as fast while they last) or half
+    const bool tall_ok = in_ok && out_ok && (slots / kTallRows + std::min(E, slots) / 2) * (long long)((std::min(d, h) + kTallCols - 1) / kTallCols) >=
+                                                (sizeof(T) == 4 ? 200 : 100);
+    // few rows per expert: tiles of 16 or 32 rows, weights streamed
+    const int few_blocks = slots <= 4 * E ? 1 : slots <= (tall_ok ? 8 : 16) * E ? 2 : 0;
+    const bool mini = few_blocks > 0 && slots <= kMiniSlots, tall = few_blocks == 0 && tall_ok;
     const int tile_rows = few_blocks > 0 ? 16 * few_blocks : tall ? kTallRows : S::kRows;
     if (!mini) {
         if (blocks > 1) plan_count_kernel<<<blocks, kPlanBlock, 4 * E, stream>>>(slots, E, ids, c.hist);

@@ -22,6 +22,7 @@ namespace {
 using namespace rows;
 
 constexpr int kFewShrink = 1024;  // rows up to which u takes waves of their own per row
+constexpr int kStreamRows = 16;   // rows up to which W is streamed in any case
 
 struct Args {
     const char *x, *w, *a, *b;
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(kStreamThreads) void shrink_kernel(Args p) {
     }
 }
 
-template <typename T, typename S, bool ALIGNED, bool B_ALIGNED>
+template <typename T, typename S, bool B_ALIGNED>
 __global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
     extern __shared__ __align__(16) char lds[];
     __shared__ int s_adapter[S::kRows], s_list[S::kRows], s_n;
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-    multiply<T, S, ALIGNED>(acc, lds, pa, pb, row_bytes);  // (starts with a barrier)
+    multiply<T, S, false>(acc, lds, pa, pb, row_bytes);  // (starts with a barrier)
 
     int mine[S::FM];
 #pragma unroll
@@ -350,12 +351,34 @@ __global__ __launch_bounds__(256) void project_join_kernel(Args p, const float* 
     reinterpret_cast<T*>(p.y + t * p.y_stride)[n] = (T)(sum + part);
 }
 
-inline int split_height(int T) { return T <= 64 ? 2 : T <= 128 ? 4 : 8; }  // FM of the tiles
-// How many workgroups share a tile's K: what 256 compute units leave room for, at least eight pairs of steps each.
-inline int split_count(int T, int d, int n, int size) {
-    const long long tiles = (long long)((T + 32 * split_height(T) - 1) / (32 * split_height(T))) * ((n + kTallCols - 1) / kTallCols);
-    const long long most = std::min<long long>(256 / tiles, (long long)d * size / (8 * kTallPair));
-    return (int)std::max<long long>(1, most);
+// Tiles of 32 * fm rows, their K cut over `splits` workgroups.
+struct Cut {
+    int fm, splits;
+};
+
+// The cut that takes least time by this model, in units of 0.2 us (what a pair of steps of one block of rows takes in 16 bits; a
+// tile's weights count as one block more): a round of up to 256 tiles costs its pairs of steps and 20 for its beginning and
+// end, a join 20 and the FP32 sums at 4 TB/s there and back.  f32 takes eight times as long a pair.  4096 x 10240: 64 rows
+// are cut (2, 6) and take 38 us, where one workgroup a tile would need 60; 1024 rows (6, 1), 240 tiles, where 160 of full height
+// or 320 of half of it need 115 to 121; 8192 rows (8, 1).
+Cut best_cut(int T, int d, int n, int size) {
+    const int pairs = ((long long)d * size + kTallPair - 1) / kTallPair, each = size == 4 ? 8 : 1;
+    const long long cols = (n + kTallCols - 1) / kTallCols;
+    Cut best{8, 1};
+    double least = 0;
+    for (int fm = 8; fm >= 2; --fm) {
+        const long long tiles = (T + 32 * fm - 1) / (32 * fm) * cols;
+        for (int s = 1; s <= 8 && (s == 1 || (pairs >= 4 * s && tiles * s <= 512)); ++s) {
+            const double rounds = (double)((tiles * s + 255) / 256);
+            const double time = rounds * ((double)(fm + 1) * each * pairs / s + 20) + (s > 1 ? 20 + (double)s * T * n / 1e5 : 0);
+            if (least == 0 || time < least) least = time, best = Cut{fm, s};
+        }
+    }
+    return best;
+}
+inline size_t sums_bytes(int T, int d, int n, int size) {
+    const int splits = T > kStreamRows ? best_cut(T, d, n, size).splits : 1;
+    return splits > 1 ? (size_t)splits * T * ((n + 3) / 4 * 4) * 4 : 0;
 }
 
 template <typename T, int FM>
@@ -367,6 +390,12 @@ hipError_t go_split(const Args& p, float* sums, int splits, bool b_aligned, hipS
     if (b_aligned) project_join_kernel<T, true><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
     else project_join_kernel<T, false><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
     return hipGetLastError();
+}
+
+template <typename T, int FM>
+hipError_t go_cut(const Args& p, float* sums, int splits, bool b_aligned, hipStream_t stream) {
+    if (splits > 1) return go_split<T, FM>(p, sums, splits, b_aligned, stream);
+    return b_aligned ? go_tall<T, FM, true>(p, stream) : go_tall<T, FM, false>(p, stream);
 }
 
 // Few rows: W streamed once through the registers, 16 * FN of its rows per workgroup; the adapters' part of an output is added
@@ -452,12 +481,12 @@ hipError_t go_few(const Args& p, bool aligned, bool b_aligned, hipStream_t strea
     return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, false, false>>{});
 }
 
-template <typename T, typename S, bool ALIGNED, bool B_ALIGNED>
+template <typename T, typename S, bool B_ALIGNED>
 hipError_t go(const Args& p, hipStream_t stream) {
     const long long grid = (long long)((p.T + S::kRows - 1) / S::kRows) * ((p.n + S::kCols - 1) / S::kCols);
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    if (const hipError_t err = allow_lds_once<project_kernel<T, S, ALIGNED, B_ALIGNED>>(S::kLds); err != hipSuccess) return err;
-    project_kernel<T, S, ALIGNED, B_ALIGNED><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
+    if (const hipError_t err = allow_lds_once<project_kernel<T, S, B_ALIGNED>>(S::kLds); err != hipSuccess) return err;
+    project_kernel<T, S, B_ALIGNED><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -482,20 +511,22 @@ hipError_t run(const Args& p, float* sums, hipStream_t stream) {
         if (a_aligned) shrink_kernel<T, FM, true><<<grid, kStreamThreads, lds, stream>>>(p);
         else shrink_kernel<T, FM, false><<<grid, kStreamThreads, lds, stream>>>(p);
     }
-    // tall tiles where there are enough of them for the compute units
-    const long long columns = (p.n + kTallCols - 1) / kTallCols;
-    if (aligned && (p.T + 255) / 256 * columns >= 200) return b_aligned ? go_tall<T, 8, true>(p, stream) : go_tall<T, 8, false>(p, stream);
-    if (aligned && (p.T + 127) / 128 * columns >= 100) return b_aligned ? go_tall<T, 4, true>(p, stream) : go_tall<T, 4, false>(p, stream);
-    if (aligned && p.T > 16) {
-        const int splits = split_count(p.T, p.d, p.n, sizeof(T));
-        if (splits > 1) {
-            if (split_height(p.T) == 2) return go_split<T, 2>(p, sums, splits, b_aligned, stream);
-            return split_height(p.T) == 4 ? go_split<T, 4>(p, sums, splits, b_aligned, stream) : go_split<T, 8>(p, sums, splits, b_aligned, stream);
+    if (aligned && p.T > kStreamRows) {
+        const Cut cut = best_cut(p.T, p.d, p.n, sizeof(T));
+        switch (cut.fm) {
+            case 2: return go_cut<T, 2>(p, sums, cut.splits, b_aligned, stream);
+            case 3: return go_cut<T, 3>(p, sums, cut.splits, b_aligned, stream);
+            case 4: return go_cut<T, 4>(p, sums, cut.splits, b_aligned, stream);
+            case 5: return go_cut<T, 5>(p, sums, cut.splits, b_aligned, stream);
+            case 6: return go_cut<T, 6>(p, sums, cut.splits, b_aligned, stream);
+            case 7: return go_cut<T, 7>(p, sums, cut.splits, b_aligned, stream);
+            default: return go_cut<T, 8>(p, sums, cut.splits, b_aligned, stream);
         }
     }
-    // Streams of up to 64 rows: W passes once per 64 rows.  The rows come through the caches, FM / FN of the weights' bytes,
-    // so as many weight rows per workgroup as leave at least 128 workgroups (64 rows by 10240 x 4096: 16 weight rows 64 us,
-    // 64 of them 26).  With more rows, as long as tiles of 64 x 128 would leave compute units without work.
+    // Up to 16 rows, and rows that are not whole 16-byte pieces: streams, W passing once per 16 to 64 rows.  The rows come
+    // through the caches, FM / FN of the weights' bytes, so as many weight rows per workgroup as leave at least 128
+    // workgroups (64 rows by 10240 x 4096: 16 weight rows 64 us, 64 of them 45).  With more rows, as long as tiles of
+    // 64 x 128 would leave compute units without work.
     const long long row_tiles = (p.T + 63) / 64;
     if (p.T <= 16) return p.n >= 32 * 512 ? go_few<T, 1, 2>(p, aligned, b_aligned, stream) : go_few<T, 1, 1>(p, aligned, b_aligned, stream);
     if (p.T <= 32) return p.n >= 32 * 128 ? go_few<T, 2, 2>(p, aligned, b_aligned, stream) : go_few<T, 2, 1>(p, aligned, b_aligned, stream);
@@ -503,8 +534,7 @@ hipError_t run(const Args& p, float* sums, hipStream_t stream) {
         if (row_tiles * ((p.n + 63) / 64) >= 128) return go_few<T, 4, 4>(p, aligned, b_aligned, stream);
         return row_tiles * ((p.n + 31) / 32) >= 128 ? go_few<T, 4, 2>(p, aligned, b_aligned, stream) : go_few<T, 4, 1>(p, aligned, b_aligned, stream);
     }
-    if (aligned) return b_aligned ? go<T, S, true, true>(p, stream) : go<T, S, true, false>(p, stream);
-    return b_aligned ? go<T, S, false, true>(p, stream) : go<T, S, false, false>(p, stream);
+    return b_aligned ? go<T, S, true>(p, stream) : go<T, S, false>(p, stream);
 }
 
 inline int u_stride_bytes(int r, int size) { return (r * size + 15) / 16 * 16; }
@@ -514,8 +544,8 @@ inline int u_stride_bytes(int r, int size) { return (r * size + 15) / 16 * 16; }
 inline size_t u_bytes(int T, int r, int size) { return ((size_t)T * u_stride_bytes(r, size) + 255) & ~(size_t)255; }
 
 size_t lora_project_workspace_bytes(int T, int d, int n, int r, int dtype) {
-    const int size = dtype == DTYPE_F32 ? 4 : 2, splits = T > 16 ? split_count(T, d, n, size) : 1;
-    return u_bytes(T, r, size) + (splits > 1 ? (size_t)splits * T * ((n + 3) / 4 * 4) * 4 : 0);
+    const int size = dtype == DTYPE_F32 ? 4 : 2;
+    return u_bytes(T, r, size) + sums_bytes(T, d, n, size);
 }
 
 hipError_t launch_lora_project(int T, int d, int n, int r, int L, int dtype, const void* x, long long x_stride, const void* w, const void* a,
