@@ -18,6 +18,10 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libinfmoe.so")
 
 SOURCES = [
+    "kernels/lora.hip",
+    "kernels/experts_topk_bf16.hip",
+    "kernels/experts_topk_f16.hip",
+    "kernels/experts_topk_f32.hip",
     "kernels/dispatch.hip",
     "kernels/norm.hip",
     # the six instantiations of the matrix-core expert kernel first: they take longest
@@ -37,7 +41,6 @@ SOURCES = [
     "kernels/expert_skinny.hip",
     "kernels/route.hip",
     "kernels/experts_topk.hip",
-    "kernels/lora.hip",
     "sublayers/t5ff_layer.cpp",
     "sublayers/sublayer.cpp",
     "npz_reader.cpp",

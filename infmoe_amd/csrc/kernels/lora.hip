@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kStreamThreads) void shrink_kernel(Args p) {
     }
 }
 
-template <typename T, typename S, bool B_ALIGNED>
+template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
     extern __shared__ __align__(16) char lds[];
     __shared__ int s_adapter[S::kRows], s_list[S::kRows], s_n;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
 #pragma unroll
         for (int i = 0; i < S::kPiecesB; ++i)
             pb[i] = p.b + ((long long)a * p.n + min(n0 + (tid >> 3) + i * (S::kThreads / 8), p.n - 1)) * r_bytes;
-        multiply_kept<T, S, B_ALIGNED>(acc, lds, pa, pb, r_bytes, keep);
+        multiply_kept<T, S, false>(acc, lds, pa, pb, r_bytes, keep);
     }
 #pragma unroll
     for (int i = 0; i < S::FM; ++i) {
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(S::kThreads) void project_kernel(Args p) {
 // adapters among its own 16 * FM rows and takes u and B_a from the caches straight into operands.
 constexpr int kTileGroup = 4;  // row tiles that share a stretch of weight columns (below)
 
-template <typename T, int FM, bool B_ALIGNED>
+template <typename T, int FM>
 __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
     extern __shared__ __align__(16) char lds[];
     using W = Tall<FM, 4>;
@@ -239,6 +239,7 @@ __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
     tall_multiply<T, FM, 4>(acc, lds, pa, pb, end);
 
     const int m = lane & 15, r_end = p.r * (int)sizeof(T);
+    const bool whole_b = ((reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)r_end) & 15) == 0;
     int mine[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
         for (int k = (lane >> 4) * 16; k - (lane >> 4) * 16 < r_end; k += 64) {
             v4u wb[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) wb[j] = k < r_end ? piece<T, B_ALIGNED>(pw[j], k, r_end) : v4u{0, 0, 0, 0};
+            for (int j = 0; j < 4; ++j) wb[j] = k >= r_end ? v4u{0, 0, 0, 0} : whole_b ? piece<T, true>(pw[j], k, r_end) : piece<T, false>(pw[j], k, r_end);
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 if (__ballot(mine[i] == a) == 0) continue;
@@ -292,12 +293,12 @@ __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
     }
 }
 
-template <typename T, int FM, bool B_ALIGNED>
+template <typename T, int FM>
 hipError_t go_tall(const Args& p, hipStream_t stream) {
     const long long all = (long long)((p.T + 32 * FM - 1) / (32 * FM)) * ((p.n + kTallCols - 1) / kTallCols);
     if (all > 0x7ffffff0) return hipErrorInvalidValue;
-    if (const hipError_t err = allow_lds_once<project_tall_kernel<T, FM, B_ALIGNED>>(kTallLds); err != hipSuccess) return err;
-    project_tall_kernel<T, FM, B_ALIGNED><<<(int)((all + kXcdCount - 1) / kXcdCount * kXcdCount), kTallThreads, kTallLds, stream>>>(p);
+    if (const hipError_t err = allow_lds_once<project_tall_kernel<T, FM>>(kTallLds); err != hipSuccess) return err;
+    project_tall_kernel<T, FM><<<(int)((all + kXcdCount - 1) / kXcdCount * kXcdCount), kTallThreads, kTallLds, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(kTallThreads) void project_split_kernel(Args p, flo
 }
 
 // (A thread per column: the lanes of a wave read rows of B_a that lie side by side.)
-template <typename T, bool B_ALIGNED>
+template <typename T>
 __global__ __launch_bounds__(256) void project_join_kernel(Args p, const float* __restrict__ sums, int splits, long long sums_stride) {
     const int t = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
     if (n >= p.n) return;
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(256) void project_join_kernel(Args p, const float* 
         const char *u = p.u + (size_t)t * p.u_stride, *b = p.b + ((long long)a * p.n + n) * r_end;
 #pragma unroll 2
         for (int k = 0; k < r_end; k += 16)  // (u is padded to whole pieces)
-            part = dot_piece<T>(*reinterpret_cast<const v4u*>(u + k), piece<T, B_ALIGNED>(b, k, r_end), part);
+            part = dot_piece<T>(*reinterpret_cast<const v4u*>(u + k), piece<T, false>(b, k, r_end), part);
     }
     reinterpret_cast<T*>(p.y + t * p.y_stride)[n] = (T)(sum + part);
 }
@@ -382,25 +383,24 @@ inline size_t sums_bytes(int T, int d, int n, int size) {
 }
 
 template <typename T, int FM>
-hipError_t go_split(const Args& p, float* sums, int splits, bool b_aligned, hipStream_t stream) {
+hipError_t go_split(const Args& p, float* sums, int splits, hipStream_t stream) {
     const long long tiles = (long long)((p.T + 32 * FM - 1) / (32 * FM)) * ((p.n + kTallCols - 1) / kTallCols), stride = (p.n + 3) / 4 * 4;
     if (const hipError_t err = allow_lds_once<project_split_kernel<T, FM>>(kTallLds); err != hipSuccess) return err;
     project_split_kernel<T, FM><<<(int)(tiles * splits), kTallThreads, kTallLds, stream>>>(p, sums, splits, stride);
     const dim3 grid((p.n + 255) / 256, p.T);
-    if (b_aligned) project_join_kernel<T, true><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
-    else project_join_kernel<T, false><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
+    project_join_kernel<T><<<grid, 256, 0, stream>>>(p, sums, splits, stride);
     return hipGetLastError();
 }
 
 template <typename T, int FM>
-hipError_t go_cut(const Args& p, float* sums, int splits, bool b_aligned, hipStream_t stream) {
-    if (splits > 1) return go_split<T, FM>(p, sums, splits, b_aligned, stream);
-    return b_aligned ? go_tall<T, FM, true>(p, stream) : go_tall<T, FM, false>(p, stream);
+hipError_t go_cut(const Args& p, float* sums, int splits, hipStream_t stream) {
+    if (splits > 1) return go_split<T, FM>(p, sums, splits, stream);
+    return go_tall<T, FM>(p, stream);
 }
 
 // Few rows: W streamed once through the registers, 16 * FN of its rows per workgroup; the adapters' part of an output is added
 // by the lane that holds the joined sum.
-template <typename T, int FM, int FN, bool ALIGNED, bool B_ALIGNED>
+template <typename T, int FM, int FN, bool ALIGNED>
 __global__ __launch_bounds__(kStreamThreads) void project_few_kernel(Args p) {
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(kStreamThreads) void project_few_kernel(Args p) {
                 const v4u uk = *reinterpret_cast<const v4u*>(u + k);  // (u is padded to whole pieces)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (n + q < p.n) part[c][q] = dot_piece<T>(uk, piece<T, B_ALIGNED>(b + q * r_end, k, r_end), part[c][q]);
+                    if (n + q < p.n) part[c][q] = dot_piece<T>(uk, piece<T, false>(b + q * r_end, k, r_end), part[c][q]);
             }
         }
     };
@@ -466,7 +466,7 @@ __global__ __launch_bounds__(kStreamThreads) void project_few_kernel(Args p) {
 }
 
 template <typename T, int FM, int FN>
-hipError_t go_few(const Args& p, bool aligned, bool b_aligned, hipStream_t stream) {
+hipError_t go_few(const Args& p, [[maybe_unused]] bool aligned, hipStream_t stream) {
     const dim3 grid((p.n + 16 * FN - 1) / (16 * FN), (p.T + 16 * FM - 1) / (16 * FM));
     constexpr int lds = stream_lds<FM, FN>();
     auto launch = [&](auto kernel) {
@@ -475,18 +475,18 @@ hipError_t go_few(const Args& p, bool aligned, bool b_aligned, hipStream_t strea
         k<<<grid, kStreamThreads, lds, stream>>>(p);
         return hipGetLastError();
     };
-    if (aligned && b_aligned) return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, true, true>>{});
-    if (aligned) return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, true, false>>{});
-    if (b_aligned) return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, false, true>>{});
-    return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, false, false>>{});
+    if constexpr (FM == 1) {  // (more rows of whole pieces go to the tall tiles)
+        if (aligned) return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, true>>{});
+    }
+    return launch(std::integral_constant<void (*)(Args), project_few_kernel<T, FM, FN, false>>{});
 }
 
-template <typename T, typename S, bool B_ALIGNED>
+template <typename T, typename S>
 hipError_t go(const Args& p, hipStream_t stream) {
     const long long grid = (long long)((p.T + S::kRows - 1) / S::kRows) * ((p.n + S::kCols - 1) / S::kCols);
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    if (const hipError_t err = allow_lds_once<project_kernel<T, S, B_ALIGNED>>(S::kLds); err != hipSuccess) return err;
-    project_kernel<T, S, B_ALIGNED><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
+    if (const hipError_t err = allow_lds_once<project_kernel<T, S>>(S::kLds); err != hipSuccess) return err;
+    project_kernel<T, S><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -495,7 +495,6 @@ hipError_t run(const Args& p, float* sums, hipStream_t stream) {
     using S = Shape<1, 4, 4, 2>;
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | p.x_stride | p.d * sizeof(T)) & 15) == 0;
     const bool a_aligned = aligned && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
-    const bool b_aligned = ((reinterpret_cast<uintptr_t>(p.b) | p.r * sizeof(T)) & 15) == 0;
     const int padded = p.u_stride / (int)sizeof(T);
     if ((long long)p.T * padded <= 4096) {
         const dim3 grid(p.T, (padded + 3) / 4);
@@ -514,13 +513,13 @@ hipError_t run(const Args& p, float* sums, hipStream_t stream) {
     if (aligned && p.T > kStreamRows) {
         const Cut cut = best_cut(p.T, p.d, p.n, sizeof(T));
         switch (cut.fm) {
-            case 2: return go_cut<T, 2>(p, sums, cut.splits, b_aligned, stream);
-            case 3: return go_cut<T, 3>(p, sums, cut.splits, b_aligned, stream);
-            case 4: return go_cut<T, 4>(p, sums, cut.splits, b_aligned, stream);
-            case 5: return go_cut<T, 5>(p, sums, cut.splits, b_aligned, stream);
-            case 6: return go_cut<T, 6>(p, sums, cut.splits, b_aligned, stream);
-            case 7: return go_cut<T, 7>(p, sums, cut.splits, b_aligned, stream);
-            default: return go_cut<T, 8>(p, sums, cut.splits, b_aligned, stream);
+            case 2: return go_cut<T, 2>(p, sums, cut.splits, stream);
+            case 3: return go_cut<T, 3>(p, sums, cut.splits, stream);
+            case 4: return go_cut<T, 4>(p, sums, cut.splits, stream);
+            case 5: return go_cut<T, 5>(p, sums, cut.splits, stream);
+            case 6: return go_cut<T, 6>(p, sums, cut.splits, stream);
+            case 7: return go_cut<T, 7>(p, sums, cut.splits, stream);
+            default: return go_cut<T, 8>(p, sums, cut.splits, stream);
         }
     }
     // Up to 16 rows, and rows that are not whole 16-byte pieces: streams, W passing once per 16 to 64 rows.  The rows come
@@ -528,13 +527,13 @@ hipError_t run(const Args& p, float* sums, hipStream_t stream) {
     // workgroups (64 rows by 10240 x 4096: 16 weight rows 64 us, 64 of them 45).  With more rows, as long as tiles of
     // 64 x 128 would leave compute units without work.
     const long long row_tiles = (p.T + 63) / 64;
-    if (p.T <= 16) return p.n >= 32 * 512 ? go_few<T, 1, 2>(p, aligned, b_aligned, stream) : go_few<T, 1, 1>(p, aligned, b_aligned, stream);
-    if (p.T <= 32) return p.n >= 32 * 128 ? go_few<T, 2, 2>(p, aligned, b_aligned, stream) : go_few<T, 2, 1>(p, aligned, b_aligned, stream);
+    if (p.T <= 16) return p.n >= 32 * 512 ? go_few<T, 1, 2>(p, aligned, stream) : go_few<T, 1, 1>(p, aligned, stream);
+    if (p.T <= 32) return p.n >= 32 * 128 ? go_few<T, 2, 2>(p, aligned, stream) : go_few<T, 2, 1>(p, aligned, stream);
     if (p.T <= 64 || row_tiles * ((p.n + 127) / 128) < 256) {
-        if (row_tiles * ((p.n + 63) / 64) >= 128) return go_few<T, 4, 4>(p, aligned, b_aligned, stream);
-        return row_tiles * ((p.n + 31) / 32) >= 128 ? go_few<T, 4, 2>(p, aligned, b_aligned, stream) : go_few<T, 4, 1>(p, aligned, b_aligned, stream);
+        if (row_tiles * ((p.n + 63) / 64) >= 128) return go_few<T, 4, 4>(p, aligned, stream);
+        return row_tiles * ((p.n + 31) / 32) >= 128 ? go_few<T, 4, 2>(p, aligned, stream) : go_few<T, 4, 1>(p, aligned, stream);
     }
-    return b_aligned ? go<T, S, true>(p, stream) : go<T, S, false>(p, stream);
+    return go<T, S>(p, stream);
 }
 
 inline int u_stride_bytes(int r, int size) { return (r * size + 15) / 16 * 16; }
