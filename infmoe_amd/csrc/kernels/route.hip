@@ -127,13 +127,17 @@ __device__ __forceinline__ bool keep_groups(const Args& a, R (&c)[V], float floo
         one = larger(one, o1);
     }
     const R value = a.group_top == 2 ? one + two : one;
+    // A group's sum is off by the errors of its scores, u |one| and u |two| of their sums with the bias, and u |value|: its terms
+    // count, not the sum in which they may cancel.  Two sums that are farther apart than 2 floor_gap + 2^-21 times the terms of
+    // either one (8 u, where 4 u times the larger would do) are ordered.
+    const R terms = a.group_top == 2 ? size_of(one) + size_of(two) : size_of(one);
     const int group = in_row >> a.lanes_log2;
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
         const R other = G == 64 ? lane_value(value, g << a.lanes_log2) : __shfl(value, (lane - in_row) + (g << a.lanes_log2));
         rank += other > value || (other == value && g < group);
         if (CHECK && g != group && group < a.groups && other > -INFINITY && value > -INFINITY)
-            sure = sure && size_of(other - value) > 2 * (R)floor_gap + (R)0x1p-21 * size_of(value);
+            sure = sure && size_of(other - value) > 2 * (R)floor_gap + (R)0x1p-21 * terms;
     }
     if (rank >= a.top_groups)
 #pragma unroll

@@ -1,0 +1,56 @@
+"""infmoe_route_topk where scores meet at a border of the choice: group sums whose terms cancel."""
+import numpy as np
+import pytest
+
+from oracle import topk_oracle as O
+
+pytestmark = pytest.mark.gpu
+RTOL = 2.0 ** -17  # of a weight; derived in test_gpu_route.py
+
+
+def check(got, want):
+    ids, w = (g.cpu().numpy() for g in got)
+    np.testing.assert_array_equal(ids, want[0])
+    np.testing.assert_allclose(w, want[1], rtol=RTOL, atol=1e-38)
+
+
+def cancelling_groups(rng, T, groups, per, score, size):
+    """Logits and a bias for which the two best of every group of `per` add up to nearly the same number, through a bias of
+    +size on the one and -size on the other; the group's other experts are far behind.  Rows in which two groups' sums lie
+    closer than 64 bits tell apart (the sums' roundings are 3 * 2^-53 * size, a score's a few 2^-53) are left out."""
+    p = np.full((T, groups, per), 0.05 / (groups * per) if score == "softmax" else 0.05)
+    pair = 0.9 / groups if score == "softmax" else 0.9
+    p[:, :, 0] = pair * rng.uniform(0.2, 0.8, (T, groups))
+    p[:, :, 1] = pair * (1 + 10.0 ** rng.uniform(-8.5, -6.5, (T, groups)) * rng.choice([-1, 1], (T, groups))) - p[:, :, 0]
+    x = (np.log(p) if score == "softmax" else np.log(p) - np.log1p(-p)).reshape(T, -1).astype(np.float32)
+    bias = np.full((groups, per), -8.0 * size, np.float32)
+    bias[:, 0], bias[:, 1] = size, -size
+    wide = x.astype(np.float64)
+    s = np.exp(wide) / np.exp(wide).sum(axis=1, keepdims=True) if score == "softmax" else 1 / (1 + np.exp(-wide))
+    sums = np.sort(s.reshape(T, groups, per)[:, :, :2].sum(axis=2), axis=1)
+    apart = np.diff(sums, axis=1).min(axis=1) > 1e-15 * (4 * size + 4)
+    assert apart.mean() > 0.9
+    return x[apart], bias.reshape(-1)
+
+
+@pytest.mark.parametrize("score,size", [("softmax", 1.0), ("softmax", 30.0), ("softmax", 300.0), ("sigmoid", 1.0), ("sigmoid", 100.0), ("sigmoid", 3e4)])
+@pytest.mark.parametrize("T,groups,top_groups,per", [(300, 2, 1, 2), (300, 8, 4, 2), (5000, 2, 1, 2), (5000, 8, 4, 32), (300, 4, 2, 64)])
+def test_group_sums_that_cancel_are_ordered_in_64_bits(lib, torch_cuda, score, size, T, groups, top_groups, per):
+    torch = torch_cuda
+    from infmoe_amd import ops
+    x, bias = cancelling_groups(np.random.default_rng(T + groups + per), T, groups, per, score, size)
+    kw = dict(score=score, groups=groups, top_groups=top_groups, group_top=2)
+    got = ops.route_topk(torch.from_numpy(x).cuda(), 2, bias=torch.from_numpy(bias).cuda(), **kw)
+    check(got, O.route_topk(x, 2, bias=bias, **kw))
+
+
+def test_a_group_sum_whose_terms_cancel(lib, torch_cuda):
+    """Group sums 0.832025 and 0.8320276 behind terms of 108: FP32's sums stand the other way round, 4e-6 apart."""
+    torch = torch_cuda
+    from infmoe_amd import ops
+    x = np.array([[0.01374958, -0.7145797, 0.4695681, -1.2847303]], np.float32)
+    bias = np.array([107.59555, -107.59555, 0, 0], np.float32)
+    kw = dict(score="sigmoid", groups=2, top_groups=1, group_top=2)
+    want = O.route_topk(x, 2, bias=bias, **kw)
+    assert want[0].tolist() == [[2, 3]]
+    check(ops.route_topk(torch.from_numpy(x).cuda(), 2, bias=torch.from_numpy(bias).cuda(), **kw), want)
