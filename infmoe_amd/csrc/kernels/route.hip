@@ -6,7 +6,7 @@
 //
 // Softmax and the logistic function keep the order of the logits, so where neither a bias nor a sum over a group enters,
 // the logits themselves are compared, which needs no arithmetic and no tolerance.  Otherwise the choice is made on scores
-// in FP32, and a row in which two neighbours of the ranking are closer than what FP32 can order (see kScoreError) is
+// in FP32, and a row in which two neighbours of the ranking are closer than what FP32 can order (see score_error) is
 // chosen once more on scores in 64 bits; a result never depends on FP32's roundings.
 //
 // Layout: a row of E logits takes a whole wave, or 16 neighbouring lanes of it when it has at most 64 experts, each lane with
@@ -92,6 +92,13 @@ __device__ __forceinline__ R row_sum(R v) {
     return v;
 }
 
+// The sum of a lane's values from I on, V of them, in pairs
+template <int I, int V, typename R, int N>
+__device__ __forceinline__ R pair_sum(const R (&v)[N]) {
+    if constexpr (V == 1) return v[I];
+    else return pair_sum<I, V / 2>(v) + pair_sum<I + V / 2, V / 2>(v);
+}
+
 __device__ __forceinline__ float load_logit(const Args& a, long long at) {
     if (a.dtype == DTYPE_F32) return static_cast<const float*>(a.logits)[at];
     const unsigned short h = static_cast<const unsigned short*>(a.logits)[at];
@@ -101,13 +108,19 @@ __device__ __forceinline__ float load_logit(const Args& a, long long at) {
 __device__ __forceinline__ float exp_of(float x) { return __expf(x); }
 
 // Two scores p + bias computed in FP32 are ordered as the exact ones when they lie further apart than
-//   kScoreError * max(p_max, 2^-10) + 2^-22 * |p + bias|.
-// exp_of(x) is 2^(x * log2 e) with the product rounded, so its relative error is at most (1.45 |x| + 2) u, u = 2^-24; a
-// logistic score p = 1 / (1 + exp(-l)) turns that into p (1 - p) (1.45 |l| + 2) u + 2 u p <= 4 u, and where all scores are
-// small, p <= 2^-10, into less than 16 u * 2^-10.  A softmax score, p = exp(l - m) / sum, has the roundings of l - m and of
-// the argument, (2.45 |l - m| + 2) u p with |l - m| p <= 0.37 p_max, those of the sum, at most (log2 E + 2) u p, and the
-// quotient's, all in all under 16 u p_max.  The sum with the bias is rounded once: u |p + bias|.  Two such errors, either way.
-constexpr float kScoreError = 0x1p-19f;  // 32 u
+//   score_error(kind) * max(p_max, 2^-10) + 2^-22 * |p + bias|.
+// exp_of(x) is 2^(x * log2 e) with the product rounded, so its relative error is at most (1.45 |x| + 2) u, u = 2^-24.
+// Logistic, p = 1 / (1 + exp(-l)): p (1 - p) (1.45 |l| + 2) u + 3 u p <= 4 u; against p_max it is largest where all scores are
+// small, (1.45 |l| + 5) u p, which from p = 2^-10 on down is at most 15 u * 2^-10.  Two such errors, either way: 30 u.
+// Softmax, p = exp(l - m) / sum:
+//   * of its own a score has the roundings of l - m and of the argument, (2.45 |l - m| + 2) u p with |l - m| p <= 0.37 p_max,
+//     and of the product with 1 / sum: under 4 u p_max;
+//   * all scores of a row share the relative error of 1 / sum: the additions, in pairs (11 at most, of up to 32 terms a lane and
+//     64 lanes; empty slots add an exact zero), the terms' errors, (2.45 a + 2) u with a the mean of |l - m| under p, which is
+//     below 4.5 for up to 1024 experts, and the quotient: under 26 u, times a difference of at most p_max.
+//   Together 26 u + 2 * 4 u = 34 u.
+// The sum with the bias is rounded once: u |p + bias|.
+__device__ __forceinline__ float score_error(int kind) { return kind == SCORE_SOFTMAX ? 0x1p-18f : 0x1p-19f; }  // 64 u, 32 u
 
 // The experts of all but the top_groups best groups masked.  R: float, or double for the rows that FP32 cannot order.  Returns
 // whether the choice of groups is certain (CHECK).
@@ -328,10 +341,10 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
         m = row_max<G>(m);
         m = m > -kInf ? m : 0.f;  // (every expert masked)
         if (scored || !a.renormalize) {
-            sum = 0.f;
+            float e[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum += exp_of(l[i] - m);
-            sum = row_sum<G>(sum);
+            for (int i = 0; i < V; ++i) e[i] = exp_of(l[i] - m);
+            sum = row_sum<G>(pair_sum<0, V>(e));
         }
     }
 
@@ -369,7 +382,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
             bad |= !(c[i] < kInf);
         }
         peak = row_max<G>(peak);
-        bool sure = choose<float, true, G, V>(a, c, kScoreError * peak, in_row, row_lanes, first, list, &mine);
+        bool sure = choose<float, true, G, V>(a, c, score_error(a.score) * peak, in_row, row_lanes, first, list, &mine);
         if (__ballot(!sure && !bad) != 0) {  // some row of this wave: all of its rows again, in 64 bits
             double d[V];
             if (a.score == SCORE_SOFTMAX) {

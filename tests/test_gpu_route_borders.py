@@ -1,4 +1,5 @@
-"""infmoe_route_topk where scores meet at a border of the choice: group sums whose terms cancel."""
+"""infmoe_route_topk where scores meet at a border of the choice: group sums whose terms cancel, a large score without a bias
+against a small one with it."""
 import numpy as np
 import pytest
 
@@ -54,3 +55,29 @@ def test_a_group_sum_whose_terms_cancel(lib, torch_cuda):
     want = O.route_topk(x, 2, bias=bias, **kw)
     assert want[0].tolist() == [[2, 3]]
     check(ops.route_topk(torch.from_numpy(x).cuda(), 2, bias=torch.from_numpy(bias).cuda(), **kw), want)
+
+
+@pytest.mark.parametrize("T,E,groups", [(300, 1024, 1), (300, 990, 33), (300, 256, 1), (5000, 256, 8), (300, 40, 1), (5000, 1023, 3)])
+@pytest.mark.parametrize("spread", [0.0, 1.0, 3.0])
+def test_a_large_score_against_a_small_one_with_a_bias(lib, torch_cuda, T, E, groups, spread):
+    """Softmax: one expert with half of the row's total against one whose bias is that half, from 1e-8 to 1e-5 apart.  The
+    error of the row's total, which all scores share, moves the one and not the other.  (`spread` of the other logits: with
+    0.0 all terms of the total are equal, and so are their roundings.)"""
+    torch = torch_cuda
+    from infmoe_amd import ops
+    rng = np.random.default_rng(E + int(10 * spread))
+    wide = spread * rng.standard_normal((T, E)) + rng.uniform(-2, 2, (T, 1))
+    wide[:, 1] -= 20.0
+    x = wide.astype(np.float32)
+    total = np.exp(x[:, 1:].astype(np.float64)).sum(axis=1)
+    near = 10.0 ** rng.uniform(-8, -5, T) * rng.choice([-1, 1], T)
+    x[:, 0] = np.log(total) + np.log((0.5 + near) / (0.5 - near))
+    bias = np.zeros(E, np.float32)
+    bias[1] = 0.5
+    s = np.exp(x.astype(np.float64))
+    s /= s.sum(axis=1, keepdims=True)
+    x = x[np.abs(s[:, 0] - s[:, 1] - 0.5) > 1e-14]  # (closer ones 64 bits do not tell apart)
+    assert len(x) > 0.9 * T
+    kw = dict(score="softmax", groups=groups, top_groups=groups)
+    got = ops.route_topk(torch.from_numpy(x).cuda(), 2, bias=torch.from_numpy(bias).cuda(), **kw)
+    check(got, O.route_topk(x, 2, bias=bias, **kw))
