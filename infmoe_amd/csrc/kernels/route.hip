@@ -163,6 +163,14 @@ __device__ __forceinline__ bool apart(float larger_one, float smaller, float flo
     return !(smaller > -kInf) || larger_one - smaller > floor_gap + 0x1p-22f * size_of(larger_one);
 }
 
+// What the lanes of this wave have written to LDS is there for the others, and nothing is moved across.  (No instruction: LDS
+// operations of one wave are done in order.  It is the compiler that must not take a lane's own store for its later load.)
+__device__ __forceinline__ void lanes_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The k best of rows of 16 lanes from a short list, when one can be had: t, the (k + 1)-th largest among the two best of every
 // lane, is reached by k + 1 experts at least and, unless many are equal or few lanes take part, by no more than 16.  Those go
 // through LDS to a lane each, in order of their indices; there every lane counts who is before it, and the counts are the
@@ -196,13 +204,16 @@ __device__ __forceinline__ bool choose_listed(const Args& a, const float (&c)[V]
     INFMOE_SCAN(0x111) INFMOE_SCAN(0x112) INFMOE_SCAN(0x114) INFMOE_SCAN(0x118)
 #undef INFMOE_SCAN
     if (__ballot(to > 16) != 0) return false;
-    float2* row = list + ((threadIdx.x & 63) >> 4) * 16;  // (one wave's LDS operations are done in order)
+    float2* row = list + ((threadIdx.x & 63) >> 4) * 16;
     row[in_row] = float2{-kInf, __int_as_float(-1)};
+    lanes_meet();  // (listed entries replace these)
     int at = to - here;
 #pragma unroll
     for (int i = 0; i < V; ++i)
         if (c[i] >= t) row[at++] = float2{c[i], __int_as_float(first + i)};
+    lanes_meet();
     const float2 entry = row[in_row];
+    lanes_meet();  // (ranked entries replace these)
     int rank = 0;
     // an equal one counts as before where its lane, and so its index, is lower
 #define INFMOE_TURN(r)                                              \
@@ -214,6 +225,7 @@ __device__ __forceinline__ bool choose_listed(const Args& a, const float (&c)[V]
 #undef INFMOE_TURN
 #undef INFMOE_EACH_TURN
     row[rank] = entry;
+    lanes_meet();
     const float2 mine_now = row[in_row];
     *mine = in_row < a.k ? __float_as_int(mine_now.y) : -1;
     const float next = dpp<0x101>(mine_now.x, -kInf);  // of the lane behind; read by all lanes, a lane that is left out gives nothing

@@ -81,3 +81,23 @@ def test_a_large_score_against_a_small_one_with_a_bias(lib, torch_cuda, T, E, gr
     kw = dict(score="softmax", groups=groups, top_groups=groups)
     got = ops.route_topk(torch.from_numpy(x).cuda(), 2, bias=torch.from_numpy(bias).cuda(), **kw)
     check(got, O.route_topk(x, 2, bias=bias, **kw))
+
+
+@pytest.mark.parametrize("E,k", [(128, 3), (128, 15), (256, 8), (200, 6)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_the_best_experts_in_a_few_lanes_of_a_row(lib, torch_cuda, E, k, score):
+    """Rows of several experts per lane whose best ones are neighbours, so that most lanes list none, up to those where one
+    lane has them all; and rows with fewer experts than k left, or with none."""
+    torch = torch_cuda
+    from infmoe_amd import ops
+    rng = np.random.default_rng(E + k)
+    T = 4100
+    x = rng.standard_normal((T, E)).astype(np.float32)
+    for t in range(T):
+        at, count = rng.integers(E), rng.integers(1, 17)
+        x[t, (at + np.arange(count)) % E] += 10.0
+    x[::17] = -np.inf
+    x[::17, 5] = np.where(rng.random(len(x[::17])) < 0.5, 1.0, -np.inf)
+    for bias in (None, (0.01 * rng.standard_normal(E)).astype(np.float32)):
+        got = ops.route_topk(torch.from_numpy(x).cuda(), k, score=score, bias=None if bias is None else torch.from_numpy(bias).cuda())
+        check(got, O.route_topk(x, k, score=score, bias=bias))
