@@ -31,10 +31,15 @@ constexpr int kTallUnit = 256 * kTallPair, kTallLds = 5 * kTallUnit;
 static __device__ const v4u kTallZeros = {0, 0, 0, 0};
 
 // 64 pieces of 16 bytes, one per lane's address, to LDS bytes [at, at + 1024) in lane order.  The transfer is in flight
-// afterwards: s_waitcnt vmcnt.  (Written out because the compiler would wait for it before any read of LDS.)
+// afterwards: s_waitcnt vmcnt.  (Written out because the compiler would wait for it before any read of LDS.  M0, which holds the
+// LDS address, is on the clobber list so that no use of it by the compiler spans the statement; that it is a register which
+// the compiler does not allocate draws a warning.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_lds(const char* from, unsigned at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // What each lane of a wave requests per pair of steps (8 rows of 128 bytes a request), and where its operands lie.  F: weight
 // operands that share a matrix (4, or 2 when half of the tile's weight rows are of a second matrix).
