@@ -415,8 +415,10 @@ int32_t infmoe_experts_topk(int32_t T, int32_t k, int32_t E, int32_t d, int32_t 
         INFMOE_NEED(T == 0 || (x && ids && weights && wi && wo && y && workspace), "experts_topk: null pointer");
         INFMOE_NEED(T == 0 || (wi_1 != nullptr) == (ffn_kind != FFN_RELU), "experts_topk: wi_1 goes with the gated kinds");
         INFMOE_NEED((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "experts_topk: workspace must be 256-byte aligned");
-        INFMOE_HIP(launch_experts_topk(T, k, E, d, h, ffn_kind, dtype, x, x_stride, ids, weights, wi, wi_1, wo, wi_stride, wo_stride, y,
-                                       y_stride, workspace, static_cast<hipStream_t>(hip_stream)));
+        const hipError_t err = launch_experts_topk(T, k, E, d, h, ffn_kind, dtype, x, x_stride, ids, weights, wi, wi_1, wo, wi_stride, wo_stride,
+                                                   y, y_stride, workspace, static_cast<hipStream_t>(hip_stream));
+        INFMOE_NEED(err != hipErrorInvalidConfiguration, "experts_topk: more tiles of rows and columns than one launch takes");
+        INFMOE_HIP(err);
         return INFMOE_OK;
     });
 }

@@ -3,7 +3,7 @@
 //
 // Launches:
 //   plan     the slots (t, j) sorted by expert (stable: results do not depend on the order anything retires in) and cut
-//            into row tiles, on the device (calls of more than kPlanBlock slots count per block first);
+//            into row tiles, on the device (calls of more than kPlanBlock slots count per block first, long ones add the counts up);
 //   product  1: rows x_t gathered by slot, activation in the epilogue, hidden rows in the weights' type;
 //   product  2: hidden rows against wo, FP32 rows in slot order;
 //   combine  the k rows of a token, weighted and added in order.
@@ -38,6 +38,10 @@ using namespace rows;
 
 constexpr int kPlanBlock = 1024;  // slots ranked by one workgroup
 constexpr int kPlanWaves = kPlanBlock / 64;
+// Blocks up to which plan_place_kernel adds the counts up itself, blocks * blocks * E of them: without the launch between, 8
+// blocks of 256 experts take 26.3 us (whole call, d = h = 32; with it 27.2), 16 blocks 31.2 (30.1), 32 blocks 41.3 (38.0), 1024
+// blocks 1680 (1160), 4096 blocks 19960 (4510).
+constexpr int kPlanScan = 16;
 constexpr int kRunTiles = 8;  // row tiles of an expert that are multiplied side by side (place_of)
 
 // ---------------------------------------------------------------- plan
@@ -50,6 +54,34 @@ __global__ __launch_bounds__(kPlanBlock) void plan_count_kernel(int S, int E, co
     if (e >= 0 && e < E) atomicAdd(&s_hist[e], 1);  // integer sums: order-free
     __syncthreads();
     for (int i = threadIdx.x; i < E; i += kPlanBlock) hist[(size_t)blockIdx.x * E + i] = s_hist[i];
+}
+
+// hist[b][e] becomes the sum of the blocks before b, hist[blocks][e] that of all.  A lane per expert, the blocks cut into a
+// stretch per wave: every wave adds up its own, then goes over it again from the sum of the stretches before it.
+__global__ __launch_bounds__(kPlanBlock) void plan_scan_kernel(int blocks, int E, int* __restrict__ hist) {
+    __shared__ int s_sum[kPlanWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+    const int b0 = (int)((long long)blocks * wave / kPlanWaves), b1 = (int)((long long)blocks * (wave + 1) / kPlanWaves);
+    int sum = 0;
+    if (e < E) {
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) sum += hist[(size_t)b * E + e];
+    }
+    s_sum[wave][lane] = sum;
+    __syncthreads();
+    if (e >= E) return;
+    int run = 0, all = 0;
+    for (int w = 0; w < kPlanWaves; ++w) {
+        run += w < wave ? s_sum[w][lane] : 0;
+        all += s_sum[w][lane];
+    }
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+        const int c = hist[(size_t)b * E + e];
+        hist[(size_t)b * E + e] = run;
+        run += c;
+    }
+    if (wave == 0) hist[(size_t)blocks * E + e] = all;
 }
 
 // Exclusive prefix of v over the workgroup's kPlanBlock threads; *total: the sum.
@@ -76,10 +108,10 @@ __device__ __forceinline__ int block_prefix(int v, int* s_wave, int* total) {
 
 // row_slot[r]: slot of the r-th row in expert order; tiles / n_tiles: its cut into tiles of at most tile_rows rows, each
 // (expert, first row, rows, place in its run | length of the run << 8).  Slots
-// whose id is no expert get no row.  Every workgroup adds up the blocks' counts itself, so that no launch lies between
-// counting and placing; one block (hist null) needs no counts of others.
+// whose id is no expert get no row.  One block (hist null) needs no counts of others; a few (scanned false) add up each other's
+// counts themselves, so that no launch lies between counting and placing; many find their prefixes in hist.
 __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(int S, int E, const int* __restrict__ ids, const int* __restrict__ hist,
-                                                                int tile_rows, int* __restrict__ row_slot, int4* __restrict__ tiles,
+                                                                bool scanned, int tile_rows, int* __restrict__ row_slot, int4* __restrict__ tiles,
                                                                 int* __restrict__ n_tiles) {
     extern __shared__ int s_dyn[];  // [kPlanWaves][E]: rows of each expert in this block, by wave
     __shared__ int s_wave[kPlanWaves];
@@ -105,6 +137,9 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(int S, int E, co
     if (i < E) {
         if (hist == nullptr) {
             for (int w = 0; w < kPlanWaves; ++w) count += s_dyn[w * E + i];
+        } else if (scanned) {
+            earlier = hist[(size_t)blockIdx.x * E + i];
+            count = hist[(size_t)gridDim.x * E + i];
         } else {
             for (int b = 0; b < (int)gridDim.x; ++b) {
                 const int c = hist[(size_t)b * E + i];
@@ -360,32 +395,33 @@ __global__ __launch_bounds__(kStreamThreads) void stream_kernel(Product p, FewRo
 // A thread per COLS columns of a token: four where there are enough of them (16-byte reads), one in small batches, where the
 // time is that of one read after the other.
 template <typename T, int COLS>
-__global__ __launch_bounds__(256) void combine_kernel(int d, int k, int E, const int* __restrict__ ids, const float* __restrict__ weights,
+__global__ __launch_bounds__(256) void combine_kernel(int T_n, int d, int k, int E, const int* __restrict__ ids, const float* __restrict__ weights,
                                                       const float* __restrict__ post, T* __restrict__ y, long long y_stride) {
     typedef float Row __attribute__((ext_vector_type(COLS)));
     struct alignas(COLS * sizeof(T)) Out {
         T e[COLS];
     };
-    const size_t t = blockIdx.x;
     const int n = (blockIdx.y * 256 + threadIdx.x) * COLS;
     if (n >= d) return;
-    float sum[COLS];
+    for (size_t t = blockIdx.x; t < (size_t)T_n; t += gridDim.x) {
+        float sum[COLS];
 #pragma unroll
-    for (int q = 0; q < COLS; ++q) sum[q] = 0.f;
+        for (int q = 0; q < COLS; ++q) sum[q] = 0.f;
 #pragma unroll 4
-    for (int j = 0; j < k; ++j) {
-        const int e = ids[t * k + j];
-        const float w = weights[t * k + j];
-        const Row v = *reinterpret_cast<const Row*>(post + (t * k + j) * d + n);  // (of a slot without an expert: never written)
+        for (int j = 0; j < k; ++j) {
+            const int e = ids[t * k + j];
+            const float w = weights[t * k + j];
+            const Row v = *reinterpret_cast<const Row*>(post + (t * k + j) * d + n);  // (of a slot without an expert: never written)
 #pragma unroll
-        for (int q = 0; q < COLS; ++q) {
-            sum[q] += w * (e >= 0 && e < E ? v[q] : 0.f);
+            for (int q = 0; q < COLS; ++q) {
+                sum[q] += w * (e >= 0 && e < E ? v[q] : 0.f);
+            }
         }
-    }
-    Out out;
+        Out out;
 #pragma unroll
-    for (int q = 0; q < COLS; ++q) out.e[q] = (T)sum[q];
-    *reinterpret_cast<Out*>(y + t * y_stride + n) = out;
+        for (int q = 0; q < COLS; ++q) out.e[q] = (T)sum[q];
+        *reinterpret_cast<Out*>(y + t * y_stride + n) = out;
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -409,7 +445,7 @@ Carve carve(int T, int k, int E, int d, int h, int dtype, char* base) {
     Carve c;
     c.row_slot = reinterpret_cast<int*>(take(4 * S));
     c.n_tiles = reinterpret_cast<int*>(take(4));
-    c.hist = reinterpret_cast<int*>(take(4 * ((S + kPlanBlock - 1) / kPlanBlock) * E));
+    c.hist = reinterpret_cast<int*>(take(4 * ((S + kPlanBlock - 1) / kPlanBlock + 1) * E));
     c.tiles = reinterpret_cast<int4*>(take(sizeof(int4) * (S / kMinTile + std::min<size_t>(E, S))));
     c.hidden = take(S * h * size);
     c.post = reinterpret_cast<float*>(take(S * d * 4));
@@ -421,7 +457,6 @@ template <typename T, typename S, bool FIRST, bool GATED>
 hipError_t go(const Product& p, int max_tiles, bool aligned, hipStream_t stream) {
     const int out = S::kCols / (GATED ? 2 : 1);
     const long long grid = ((long long)max_tiles * ((p.N + out - 1) / out) + kXcdCount - 1) / kXcdCount * kXcdCount;
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
     if (aligned) {
         if (const hipError_t err = allow_lds_once<product_kernel<T, S, FIRST, GATED, true>>(S::kLds); err != hipSuccess) return err;
         product_kernel<T, S, FIRST, GATED, true><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
@@ -436,7 +471,6 @@ template <typename T, bool FIRST, bool GATED>
 hipError_t go_tall(const Product& p, int max_tiles, hipStream_t stream) {
     constexpr int out = GATED ? kTallCols / 2 : kTallCols;
     const long long grid = ((long long)max_tiles * ((p.N + out - 1) / out) + kXcdCount - 1) / kXcdCount * kXcdCount;
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
     if (const hipError_t err = allow_lds_once<tall_kernel<T, FIRST, GATED>>(kTallLds); err != hipSuccess) return err;
     tall_kernel<T, FIRST, GATED><<<(int)grid, kTallThreads, kTallLds, stream>>>(p);
     return hipGetLastError();
@@ -446,7 +480,6 @@ template <typename T, int FM, int FN, bool FIRST, bool GATED>
 hipError_t go_stream(const Product& p, const FewRows& few, int max_tiles, bool aligned, hipStream_t stream) {
     constexpr int out = 16 * FN / (GATED ? 2 : 1), lds = stream_lds<FM, FN>();
     const long long grid = (long long)max_tiles * ((p.N + out - 1) / out);
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
     if (aligned) {
         if (const hipError_t err = allow_lds_once<stream_kernel<T, FM, FN, FIRST, GATED, true>>(lds); err != hipSuccess) return err;
         stream_kernel<T, FM, FN, FIRST, GATED, true><<<(int)grid, kStreamThreads, lds, stream>>>(p, few);
@@ -484,13 +517,18 @@ hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long lon
     const int few_blocks = slots <= 4 * E ? 1 : slots <= (tall_ok ? 8 : 16) * E ? 2 : 0;
     const bool mini = few_blocks > 0 && slots <= kMiniSlots, tall = few_blocks == 0 && tall_ok;
     const int tile_rows = few_blocks > 0 ? 16 * few_blocks : tall ? kTallRows : S::kRows;
+    const int max_tiles = (mini ? 0 : slots / tile_rows) + std::min(E, slots);
+    // a launch has fewer than 2^32 work items in x (where a streamed product has that many, go_few takes 64 weight rows each)
+    const int out = few_blocks > 0 ? 64 : tall ? kTallCols : S::kCols, threads = few_blocks > 0 ? kStreamThreads : tall ? kTallThreads : S::kThreads;
+    auto items = [&](int N, int each) { return ((long long)max_tiles * ((N + each - 1) / each) + kXcdCount) * threads; };
+    if (items(h, ffn == FFN_RELU ? out : out / 2) >= 1ll << 32 || items(d, out) >= 1ll << 32) return hipErrorInvalidConfiguration;
     if (!mini) {
         if (blocks > 1) plan_count_kernel<<<blocks, kPlanBlock, 4 * E, stream>>>(slots, E, ids, c.hist);
+        if (blocks > kPlanScan) plan_scan_kernel<<<(E + 63) / 64, kPlanBlock, 0, stream>>>(blocks, E, c.hist);
         const size_t lds = 4 * (size_t)kPlanWaves * E;
         if (const hipError_t err = allow_lds_once<plan_place_kernel>(4 * kPlanWaves * kRouteMaxExperts); err != hipSuccess) return err;
-        plan_place_kernel<<<blocks, kPlanBlock, lds, stream>>>(slots, E, ids, blocks > 1 ? c.hist : nullptr, tile_rows, c.row_slot, c.tiles, c.n_tiles);
+        plan_place_kernel<<<blocks, kPlanBlock, lds, stream>>>(slots, E, ids, blocks > 1 ? c.hist : nullptr, blocks > kPlanScan, tile_rows, c.row_slot, c.tiles, c.n_tiles);
     }
-    const int max_tiles = (mini ? 0 : slots / tile_rows) + std::min(E, slots);
     const FewRows few{mini ? ids : nullptr, slots, E};
     Product p{};
     p.row_slot = c.row_slot, p.tiles = c.tiles, p.n_tiles = c.n_tiles, p.k_slots = k, p.ffn = ffn;
@@ -518,8 +556,9 @@ hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long lon
                             : go<T, S, false, false>(p, max_tiles, out_ok, stream);
     if (err != hipSuccess) return err;
     const bool wide = d % 4 == 0 && (long long)Tn * d >= 1 << 20 && ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(y_stride * (long long)sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
-    if (wide) combine_kernel<T, 4><<<dim3(Tn, (d + 1023) / 1024), 256, 0, stream>>>(d, k, E, ids, weights, c.post, y, y_stride);
-    else combine_kernel<T, 1><<<dim3(Tn, (d + 255) / 256), 256, 0, stream>>>(d, k, E, ids, weights, c.post, y, y_stride);
+    const int tokens = std::min(Tn, 1 << 22);  // (a launch has fewer than 2^32 work items in x)
+    if (wide) combine_kernel<T, 4><<<dim3(tokens, (d + 1023) / 1024), 256, 0, stream>>>(Tn, d, k, E, ids, weights, c.post, y, y_stride);
+    else combine_kernel<T, 1><<<dim3(tokens, (d + 255) / 256), 256, 0, stream>>>(Tn, d, k, E, ids, weights, c.post, y, y_stride);
     return hipGetLastError();
 }
 

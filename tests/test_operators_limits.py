@@ -1,0 +1,18 @@
+"""Sizes that the operators for several experts per token cannot launch are refused before anything is; no GPU is touched."""
+import pytest
+
+from infmoe_amd import capi
+from tests.test_operators_host import experts
+
+
+@pytest.mark.parametrize("change", [
+    dict(T=1 << 25, k=32, h=1 << 20, wi_stride=1 << 24, wo_stride=1 << 24),
+    dict(T=1 << 30, k=1, d=1024, h=64, x_stride=1024, y_stride=1024, wi_stride=1 << 16, wo_stride=1 << 16),
+    dict(T=1 << 30, k=1, d=1024, h=1024, dtype=2, x_stride=1024, y_stride=1024, wi_stride=1 << 20, wo_stride=1 << 20),
+    dict(T=64, k=16, E=1024, h=1 << 23, wi_stride=1 << 27, wo_stride=1 << 27),
+    dict(T=64, k=16, E=1024, d=1 << 23, x_stride=1 << 23, y_stride=1 << 23, wi_stride=1 << 28, wo_stride=1 << 28),
+    dict(T=1 << 26, k=16, E=2, d=13, h=29),
+])
+def test_experts_refuse_more_tiles_than_a_launch_holds(change):
+    assert experts(**change) == capi.ERR_INVALID_ARGUMENT
+    assert b"experts_topk: more tiles" in capi.load().infmoe_last_error()
