@@ -440,10 +440,18 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
 }
 
 template <int G, int V>
-hipError_t go(const Args& a, hipStream_t stream) {
-    const int rows = kThreads / G;
-    route_kernel<G, V><<<(a.T + rows - 1) / rows, kThreads, 0, stream>>>(a);
-    return hipGetLastError();
+hipError_t go(const Args& all, hipStream_t stream) {
+    constexpr int rows = kThreads / G, most = (1 << 23) * rows;  // (a launch has fewer than 2^32 work items)
+    Args a = all;
+    for (int done = 0;;) {
+        a.T = min(all.T - done, most);
+        route_kernel<G, V><<<(a.T - 1) / rows + 1, kThreads, 0, stream>>>(a);
+        if (a.T == all.T - done) return hipGetLastError();
+        done += a.T;
+        a.logits = static_cast<const char*>(a.logits) + a.T * a.stride * (a.dtype == DTYPE_F32 ? 4 : 2);
+        a.ids += (size_t)a.T * a.k;
+        a.weights += (size_t)a.T * a.k;
+    }
 }
 
 template <int G>

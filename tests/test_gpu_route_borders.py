@@ -101,3 +101,24 @@ def test_the_best_experts_in_a_few_lanes_of_a_row(lib, torch_cuda, E, k, score):
     for bias in (None, (0.01 * rng.standard_normal(E)).astype(np.float32)):
         got = ops.route_topk(torch.from_numpy(x).cuda(), k, score=score, bias=None if bias is None else torch.from_numpy(bias).cuda())
         check(got, O.route_topk(x, k, score=score, bias=bias))
+
+
+@pytest.mark.parametrize("T,E,k", [((1 << 31) - 1, 1, 1), ((1 << 26) + 77, 20, 17), ((1 << 27) + 77, 2, 1)])
+def test_more_rows_than_one_launch_has_work_items_for(lib, torch_cuda, T, E, k):
+    """Rows of 16 lanes and of 64 beyond 2^32 work items, and the largest count there is.  Every row is one of 1000."""
+    torch = torch_cuda
+    from infmoe_amd import ops
+    rng = np.random.default_rng(E)
+    x = rng.standard_normal((1000, E)).astype(np.float16)
+    ids, w = O.route_topk(x.astype(np.float32), k, renormalize=False)
+    ids, w = torch.from_numpy(ids).cuda(), torch.from_numpy(w.astype(np.float32)).cuda()
+    row = lambda start, stop: torch.arange(start, stop, device="cuda") * 7 % 1000
+    logits = torch.empty(T, E, dtype=torch.float16, device="cuda")
+    table, step = torch.from_numpy(x).cuda(), 1 << 26
+    for at in range(0, T, step):
+        logits[at:at + step] = table[row(at, min(at + step, T))]
+    got_ids, got_w = ops.route_topk(logits, k, renormalize=False)
+    for at in range(0, T, step):
+        r = row(at, min(at + step, T))
+        assert torch.equal(got_ids[at:at + step], ids[r])
+        assert ((got_w[at:at + step] - w[r]).abs() <= RTOL * w[r]).all()
