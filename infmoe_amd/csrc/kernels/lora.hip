@@ -296,7 +296,6 @@ __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
 template <typename T, int FM>
 hipError_t go_tall(const Args& p, hipStream_t stream) {
     const long long all = (long long)((p.T + 32 * FM - 1) / (32 * FM)) * ((p.n + kTallCols - 1) / kTallCols);
-    if (all > 0x7ffffff0) return hipErrorInvalidValue;
     if (const hipError_t err = allow_lds_once<project_tall_kernel<T, FM>>(kTallLds); err != hipSuccess) return err;
     project_tall_kernel<T, FM><<<(int)((all + kXcdCount - 1) / kXcdCount * kXcdCount), kTallThreads, kTallLds, stream>>>(p);
     return hipGetLastError();
@@ -368,7 +367,7 @@ Cut best_cut(int T, int d, int n, int size) {
     Cut best{8, 1};
     double least = 0;
     for (int fm = 8; fm >= 2; --fm) {
-        const long long tiles = (T + 32 * fm - 1) / (32 * fm) * cols;
+        const long long tiles = (T + 32ll * fm - 1) / (32 * fm) * cols;
         for (int s = 1; s <= 8 && (s == 1 || (pairs >= 4 * s && tiles * s <= 512)); ++s) {
             const double rounds = (double)((tiles * s + 255) / 256);
             const double time = rounds * ((double)(fm + 1) * each * pairs / s + 20) + (s > 1 ? 20 + (double)s * T * n / 1e5 : 0);
@@ -484,7 +483,6 @@ hipError_t go_few(const Args& p, [[maybe_unused]] bool aligned, hipStream_t stre
 template <typename T, typename S>
 hipError_t go(const Args& p, hipStream_t stream) {
     const long long grid = (long long)((p.T + S::kRows - 1) / S::kRows) * ((p.n + S::kCols - 1) / S::kCols);
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
     if (const hipError_t err = allow_lds_once<project_kernel<T, S>>(S::kLds); err != hipSuccess) return err;
     project_kernel<T, S><<<(int)grid, S::kThreads, S::kLds, stream>>>(p);
     return hipGetLastError();
@@ -556,9 +554,22 @@ hipError_t launch_lora_project(int T, int d, int n, int r, int L, int dtype, con
     const Args p{in(x), in(w), in(a), in(b), static_cast<char*>(workspace), static_cast<char*>(y), adapter, scale, x_stride * size, y_stride * size,
                  T, d, n, r, L, u_stride_bytes(r, size)};
     float* sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + u_bytes(T, r, size));
-    if (dtype == DTYPE_F32) return run<float>(p, sums, stream);
-    if (dtype == DTYPE_F16) return run<_Float16>(p, sums, stream);
-    return run<__bf16>(p, sums, stream);
+    // A launch has fewer than 2^32 work items in x: at most 2^26 rows (the adapters' first product has 16 a row), and fewer than
+    // 2^24 tiles of 64 x 128 with 256 work items each (tall ones have no more).  Beyond, the rows go in equal parts, none of which
+    // is so short that its K would be cut.
+    const long long most = std::min(1ll << 26, ((1 << 24) - 64) / ((n + 255) / 256 * 2) * 64ll);
+    const int parts = (int)((T - 1) / most) + 1;
+    for (int i = 0; i < parts; ++i) {
+        const long long from = (long long)T * i / parts, to = (long long)T * (i + 1) / parts;
+        Args part = p;
+        part.T = (int)(to - from);
+        part.x += from * p.x_stride, part.y += from * p.y_stride, part.u += from * p.u_stride, part.adapter += from;
+        const hipError_t err = dtype == DTYPE_F32   ? run<float>(part, sums, stream)
+                               : dtype == DTYPE_F16 ? run<_Float16>(part, sums, stream)
+                                                    : run<__bf16>(part, sums, stream);
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
 }
 
 }  // namespace infmoe
