@@ -394,9 +394,10 @@ int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const 
     });
 }
 
-// (sizes that are refused below get zero)
+// (what a call cannot ask for gets zero, so that no caller allocates for it)
 size_t infmoe_experts_topk_workspace_bytes(int32_t T, int32_t k, int32_t E, int32_t d, int32_t h, int32_t dtype) {
-    if (T <= 0 || k <= 0 || E <= 0 || d <= 0 || h <= 0) return 0;
+    if (T <= 0 || k <= 0 || k > kRouteMaxTopK || E <= 0 || E > kRouteMaxExperts || (int64_t)T * k > (1 << 30)) return 0;
+    if (d <= 0 || h <= 0 || d > kRowsMaxLength || h > kRowsMaxLength || dtype < DTYPE_F32 || dtype > DTYPE_BF16) return 0;
     return experts_topk_workspace_bytes(T, k, E, d, h, dtype);
 }
 
@@ -424,7 +425,8 @@ int32_t infmoe_experts_topk(int32_t T, int32_t k, int32_t E, int32_t d, int32_t 
 }
 
 size_t infmoe_lora_project_workspace_bytes(int32_t T, int32_t d, int32_t n, int32_t r, int32_t dtype) {
-    if (T <= 0 || d <= 0 || n <= 0 || r <= 0) return 0;
+    if (T <= 0 || d <= 0 || n <= 0 || d > kRowsMaxLength || n > kRowsMaxLength) return 0;
+    if (r <= 0 || r > kLoraMaxRank || dtype < DTYPE_F32 || dtype > DTYPE_BF16) return 0;
     return lora_project_workspace_bytes(T, d, n, r, dtype);
 }
 

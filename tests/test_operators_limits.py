@@ -16,3 +16,16 @@ from tests.test_operators_host import experts
 def test_experts_refuse_more_tiles_than_a_launch_holds(change):
     assert experts(**change) == capi.ERR_INVALID_ARGUMENT
     assert b"experts_topk: more tiles" in capi.load().infmoe_last_error()
+
+
+@pytest.mark.parametrize("sizes", [
+    (4, 33, 8, 16, 24, 0), (4, 2, 1025, 16, 24, 0), (1 << 30, 2, 8, 16, 24, 0), ((1 << 31) - 1, 32, 1024, 1 << 23, 1 << 23, 0),
+    (4, 2, 8, (1 << 23) + 1, 24, 0), (4, 2, 8, 16, (1 << 31) - 1, 2), (4, 2, 8, 16, 24, 3), (4, 2, 8, 16, 24, -1)])
+def test_no_workspace_for_experts_that_are_refused(sizes):
+    assert capi.load().infmoe_experts_topk_workspace_bytes(*sizes) == 0
+
+
+@pytest.mark.parametrize("sizes", [
+    (4, (1 << 23) + 1, 24, 4, 0), (4, 16, (1 << 31) - 1, 4, 0), (4, 16, 24, 257, 0), (4, 16, 24, (1 << 31) - 1, 0), (4, 16, 24, 4, 3), (4, 16, 24, 4, -1)])
+def test_no_workspace_for_adapters_that_are_refused(sizes):
+    assert capi.load().infmoe_lora_project_workspace_bytes(*sizes) == 0
