@@ -377,7 +377,7 @@ Cut best_cut(int T, int d, int n, int size) {
     return best;
 }
 inline size_t sums_bytes(int T, int d, int n, int size) {
-    const int splits = T > kStreamRows ? best_cut(T, d, n, size).splits : 1;
+    const int splits = T > kStreamRows && (size_t)d * size % 16 == 0 ? best_cut(T, d, n, size).splits : 1;
     return splits > 1 ? (size_t)splits * T * ((n + 3) / 4 * 4) * 4 : 0;
 }
 

@@ -29,3 +29,13 @@ def test_no_workspace_for_experts_that_are_refused(sizes):
     (4, (1 << 23) + 1, 24, 4, 0), (4, 16, (1 << 31) - 1, 4, 0), (4, 16, 24, 257, 0), (4, 16, 24, (1 << 31) - 1, 0), (4, 16, 24, 4, 3), (4, 16, 24, 4, -1)])
 def test_no_workspace_for_adapters_that_are_refused(sizes):
     assert capi.load().infmoe_lora_project_workspace_bytes(*sizes) == 0
+
+
+@pytest.mark.parametrize("dtype,size", [(0, 4), (1, 2), (2, 2)])
+@pytest.mark.parametrize("T", [64, 300])
+def test_partial_sums_only_for_rows_of_whole_pieces(dtype, size, T):
+    """K is cut over workgroups for rows of whole 16-byte pieces only; others need no more than the adapters' first product."""
+    bytes_of = capi.load().infmoe_lora_project_workspace_bytes
+    first = (T * 16 * size + 255) // 256 * 256
+    assert bytes_of(T, 4096, 1024, 16, dtype) > first
+    assert bytes_of(T, 4097, 1024, 16, dtype) == first
