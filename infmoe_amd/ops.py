@@ -2,7 +2,8 @@
 
 Thin calls of the C ABI (include/infmoe.h has the definitions and limits): torch gives device memory and the current stream
 of the tensors' device, libinfmoe.so computes.  Outputs are new tensors unless `out` is given; workspaces come from torch's
-allocator per call, so concurrent streams and captured graphs never share one.
+allocator per call, so concurrent streams and captured graphs never share one.  There is no backward pass: tensors that require a
+gradient are refused unless gradients are off (torch.no_grad(), torch.inference_mode()).
 """
 from __future__ import annotations
 
@@ -25,6 +26,13 @@ def _load():
 
 def _refuse(message: str) -> None:
     raise capi.InfMoEError(capi.ERR_INVALID_ARGUMENT, message)
+
+
+def _forward_only(*tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _refuse("an input requires a gradient, which these operators do not give: detach it or call under torch.no_grad()")
 
 
 def _start(name: str, t: torch.Tensor) -> Tuple[int, int, int, int]:
@@ -66,6 +74,7 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Op
 
     score: "softmax" or "sigmoid"; bias: float32 [E], added to the scores for the choice only; groups > 1: only the
     top_groups groups with the largest sums of their group_top best experts stay.  See infmoe_route_topk."""
+    _forward_only(logits, bias, *(out or ()))
     T, E, stride, dtype = _start("logits", logits)
     device = logits.device
     kind = capi.SCORE_KINDS.get(score)
@@ -113,6 +122,7 @@ def experts_topk(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, wi: 
 
     ffn: "relu", "gated_gelu" or "gated_silu" (the gated ones take wi_1).  An id that is no expert adds nothing.  See
     infmoe_experts_topk."""
+    _forward_only(x, weights, wi, wo, wi_1, out)
     T, d, x_stride, dtype = _start("x", x)
     device, kind = x.device, capi.TOPK_FFN_KINDS.get(ffn)
     if kind is None:
@@ -139,6 +149,7 @@ def lora_project(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Ten
                  scale: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] = w x[t] + scale[i] * b[i] (a[i] x[t]) with i = adapter[t]: x [T, d], w [n, d], a [L, r, d], b [L, n, r], adapter int32
     [T], scale float32 [L] -> [T, n].  A row whose adapter is none of the L gets w x[t].  See infmoe_lora_project."""
+    _forward_only(x, w, a, b, scale, out)
     T, d, x_stride, dtype = _start("x", x)
     device = x.device
     if w.dim() != 2 or a.dim() != 3:
