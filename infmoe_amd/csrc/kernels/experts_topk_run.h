@@ -26,6 +26,7 @@
 
 #include <algorithm>
 
+#include "forms.h"
 #include "kernels.h"
 #include "row_gemm.h"
 #include "row_stream.h"
@@ -35,6 +36,7 @@ namespace infmoe {
 namespace {
 
 using namespace rows;
+using forms::kMiniSlots;
 
 constexpr int kPlanBlock = 1024;  // slots ranked by one workgroup
 constexpr int kPlanWaves = kPlanBlock / 64;
@@ -314,8 +316,6 @@ __global__ __launch_bounds__(kTallThreads) void tall_kernel(Product p) {
 // Hidden rows in slot order here, so that calls of up to kMiniSlots slots need no plan: every wave finds the slots of its
 // expert among the ids by ballots.  (Up to 64 slots are one ballot; the t-th expert in use is that of the t-th slot whose
 // expert does not occur before it.)
-constexpr int kMiniSlots = 64;
-
 struct FewRows {
     const int* ids;
     int S, E;  // ids: null when there is a plan
@@ -490,13 +490,11 @@ hipError_t go_stream(const Product& p, const FewRows& few, int max_tiles, bool a
     return hipGetLastError();
 }
 
-// Weight rows per workgroup: 64 (32 hidden columns of a gated product) where that leaves every compute unit two workgroups,
-// down to 16 otherwise.
 template <typename T, int FM, bool FIRST, bool GATED>
 hipError_t go_few(const Product& p, const FewRows& few, int max_tiles, bool aligned, hipStream_t stream) {
-    const long long blocks16 = (long long)max_tiles * ((p.N + 15) / 16) * (GATED ? 2 : 1);
-    if (blocks16 >= 4 * 512) return go_stream<T, FM, 4, FIRST, GATED>(p, few, max_tiles, aligned, stream);
-    if (GATED || blocks16 >= 2 * 512) return go_stream<T, FM, 2, FIRST, GATED>(p, few, max_tiles, aligned, stream);
+    const int fn = forms::stream_blocks(max_tiles, p.N, GATED);
+    if (fn == 4) return go_stream<T, FM, 4, FIRST, GATED>(p, few, max_tiles, aligned, stream);
+    if (GATED || fn == 2) return go_stream<T, FM, 2, FIRST, GATED>(p, few, max_tiles, aligned, stream);
     if constexpr (!GATED) return go_stream<T, FM, 1, FIRST, GATED>(p, few, max_tiles, aligned, stream);
     return hipErrorInvalidValue;
 }
@@ -510,14 +508,10 @@ hipError_t run(int Tn, int k, int E, int d, int h, int ffn, const T* x, long lon
     auto on16 = [](const void* p, long long stride) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (long long)sizeof(T))) & 15) == 0; };
     const bool in_ok = d * sizeof(T) % 16 == 0 && on16(x, x_stride) && on16(wi, wi_stride) && on16(wi_1, 0);
     const bool out_ok = h * sizeof(T) % 16 == 0 && on16(wo, wo_stride);
-    // tall tiles, if about as many as compute units can be expected (f32, whose small tiles are as fast while they last) or half
-    const bool tall_ok = in_ok && out_ok && (slots / kTallRows + std::min(E, slots) / 2) * (long long)((std::min(d, h) + kTallCols - 1) / kTallCols) >=
-                                                (sizeof(T) == 4 ? 200 : 100);
-    // few rows per expert: tiles of 16 or 32 rows, weights streamed
-    const int few_blocks = slots <= 4 * E ? 1 : slots <= (tall_ok ? 8 : 16) * E ? 2 : 0;
-    const bool mini = few_blocks > 0 && slots <= kMiniSlots, tall = few_blocks == 0 && tall_ok;
-    const int tile_rows = few_blocks > 0 ? 16 * few_blocks : tall ? kTallRows : S::kRows;
-    const int max_tiles = (mini ? 0 : slots / tile_rows) + std::min(E, slots);
+    const forms::Experts form = forms::experts_form(slots, E, d, h, sizeof(T), in_ok && out_ok);
+    static_assert(forms::kTallTileRows == kTallRows && forms::kTallCutCols == kTallCols && forms::kSmallTileRows == S::kRows, "the tiles that forms.h counts");
+    const int few_blocks = form.blocks, tile_rows = form.tile_rows, max_tiles = form.max_tiles;
+    const bool mini = form.mini, tall = form.kind == forms::Experts::TALL;
     // a launch has fewer than 2^32 work items in x (where a streamed product has that many, go_few takes 64 weight rows each)
     const int out = few_blocks > 0 ? 64 : tall ? kTallCols : S::kCols, threads = few_blocks > 0 ? kStreamThreads : tall ? kTallThreads : S::kThreads;
     auto items = [&](int N, int each) { return ((long long)max_tiles * ((N + each - 1) / each) + kXcdCount) * threads; };

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 
+#include "forms.h"
 #include "kernels.h"
 #include "row_gemm.h"
 #include "row_stream.h"
@@ -20,9 +21,7 @@ namespace infmoe {
 namespace {
 
 using namespace rows;
-
-constexpr int kFewShrink = 1024;  // rows up to which u takes waves of their own per row
-constexpr int kStreamRows = 16;   // rows up to which W is streamed in any case
+static_assert(forms::kTallCutCols == kTallCols && forms::kTallCutBytes == kTallPair, "the tiles that forms.h counts");
 
 struct Args {
     const char *x, *w, *a, *b;
@@ -302,7 +301,7 @@ hipError_t go_tall(const Args& p, hipStream_t stream) {
 }
 
 // Rows too few for tall tiles to fill the compute units: the tiles' K is cut over `splits` workgroups, each of which leaves FP32
-// sums, and a second launch adds them and the adapters' part.  (64 rows by 10240 x 4096: 40 tiles, cut in six.  Streamed by
+// sums, and a second launch adds them and the adapters' part.  (64 rows by 10240 x 4096: 40 tiles, cut in five.  Streamed by
 // project_few_kernel the rows pass every compute unit's cache once per 64 weight rows, half of all bytes: 39 us.)
 template <typename T, int FM>
 __global__ __launch_bounds__(kTallThreads) void project_split_kernel(Args p, float* __restrict__ sums, int splits, long long sums_stride) {
@@ -351,33 +350,8 @@ __global__ __launch_bounds__(256) void project_join_kernel(Args p, const float* 
     reinterpret_cast<T*>(p.y + t * p.y_stride)[n] = (T)(sum + part);
 }
 
-// Tiles of 32 * fm rows, their K cut over `splits` workgroups.
-struct Cut {
-    int fm, splits;
-};
-
-// The cut that takes least time by this model, in units of 0.2 us (what a pair of steps of one block of rows takes in 16 bits; a
-// tile's weights count as one block more): a round of up to 256 tiles costs its pairs of steps and 20 for its beginning and
-// end, a join 20 and the FP32 sums at 4 TB/s there and back.  f32 takes eight times as long a pair.  4096 x 10240: 64 rows
-// are cut (2, 6) and take 38 us, where one workgroup a tile would need 60; 1024 rows (6, 1), 240 tiles, where 160 of full height
-// or 320 of half of it need 115 to 121; 8192 rows (8, 1).
-Cut best_cut(int T, int d, int n, int size) {
-    const int pairs = ((long long)d * size + kTallPair - 1) / kTallPair, each = size == 4 ? 8 : 1;
-    const long long cols = (n + kTallCols - 1) / kTallCols;
-    Cut best{8, 1};
-    double least = 0;
-    for (int fm = 8; fm >= 2; --fm) {
-        const long long tiles = (T + 32ll * fm - 1) / (32 * fm) * cols;
-        for (int s = 1; s <= 8 && (s == 1 || (pairs >= 4 * s && tiles * s <= 512)); ++s) {
-            const double rounds = (double)((tiles * s + 255) / 256);
-            const double time = rounds * ((double)(fm + 1) * each * pairs / s + 20) + (s > 1 ? 20 + (double)s * T * n / 1e5 : 0);
-            if (least == 0 || time < least) least = time, best = Cut{fm, s};
-        }
-    }
-    return best;
-}
 inline size_t sums_bytes(int T, int d, int n, int size) {
-    const int splits = T > kStreamRows && (size_t)d * size % 16 == 0 ? best_cut(T, d, n, size).splits : 1;
+    const int splits = forms::project_form(T, d, n, size, (size_t)d * size % 16 == 0).splits;
     return splits > 1 ? (size_t)splits * T * ((n + 3) / 4 * 4) * 4 : 0;
 }
 
@@ -494,44 +468,49 @@ hipError_t run(const Args& p, float* sums, hipStream_t stream) {
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | p.x_stride | p.d * sizeof(T)) & 15) == 0;
     const bool a_aligned = aligned && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
     const int padded = p.u_stride / (int)sizeof(T);
-    if ((long long)p.T * padded <= 4096) {
-        const dim3 grid(p.T, (padded + 3) / 4);
-        if (a_aligned) shrink_few_kernel<T, 1, true><<<grid, 256, 0, stream>>>(p);
-        else shrink_few_kernel<T, 1, false><<<grid, 256, 0, stream>>>(p);
-    } else if (p.T <= kFewShrink) {
-        const dim3 grid(p.T, (padded + 15) / 16);
-        if (a_aligned) shrink_few_kernel<T, 4, true><<<grid, 256, 0, stream>>>(p);
-        else shrink_few_kernel<T, 4, false><<<grid, 256, 0, stream>>>(p);
-    } else {
-        constexpr int FM = 2, lds = stream_lds<FM, 2>();
-        const dim3 grid((p.T + 16 * FM - 1) / (16 * FM), (p.r + 31) / 32);
-        if (a_aligned) shrink_kernel<T, FM, true><<<grid, kStreamThreads, lds, stream>>>(p);
-        else shrink_kernel<T, FM, false><<<grid, kStreamThreads, lds, stream>>>(p);
-    }
-    if (aligned && p.T > kStreamRows) {
-        const Cut cut = best_cut(p.T, p.d, p.n, sizeof(T));
-        switch (cut.fm) {
-            case 2: return go_cut<T, 2>(p, sums, cut.splits, stream);
-            case 3: return go_cut<T, 3>(p, sums, cut.splits, stream);
-            case 4: return go_cut<T, 4>(p, sums, cut.splits, stream);
-            case 5: return go_cut<T, 5>(p, sums, cut.splits, stream);
-            case 6: return go_cut<T, 6>(p, sums, cut.splits, stream);
-            case 7: return go_cut<T, 7>(p, sums, cut.splits, stream);
-            default: return go_cut<T, 8>(p, sums, cut.splits, stream);
+    switch (forms::shrink_form(p.T, padded)) {
+        case forms::Shrink::ONE_RANK: {
+            const dim3 grid(p.T, (padded + 3) / 4);
+            if (a_aligned) shrink_few_kernel<T, 1, true><<<grid, 256, 0, stream>>>(p);
+            else shrink_few_kernel<T, 1, false><<<grid, 256, 0, stream>>>(p);
+            break;
+        }
+        case forms::Shrink::FOUR_RANKS: {
+            const dim3 grid(p.T, (padded + 15) / 16);
+            if (a_aligned) shrink_few_kernel<T, 4, true><<<grid, 256, 0, stream>>>(p);
+            else shrink_few_kernel<T, 4, false><<<grid, 256, 0, stream>>>(p);
+            break;
+        }
+        case forms::Shrink::TILES: {
+            constexpr int FM = 2, lds = stream_lds<FM, 2>();
+            const dim3 grid((p.T + 16 * FM - 1) / (16 * FM), (p.r + 31) / 32);
+            if (a_aligned) shrink_kernel<T, FM, true><<<grid, kStreamThreads, lds, stream>>>(p);
+            else shrink_kernel<T, FM, false><<<grid, kStreamThreads, lds, stream>>>(p);
+            break;
         }
     }
-    // Up to 16 rows, and rows that are not whole 16-byte pieces: streams, W passing once per 16 to 64 rows.  The rows come
-    // through the caches, FM / FN of the weights' bytes, so as many weight rows per workgroup as leave at least 128
-    // workgroups (64 rows by 10240 x 4096: 16 weight rows 64 us, 64 of them 45).  With more rows, as long as tiles of
-    // 64 x 128 would leave compute units without work.
-    const long long row_tiles = (p.T + 63) / 64;
-    if (p.T <= 16) return p.n >= 32 * 512 ? go_few<T, 1, 2>(p, aligned, stream) : go_few<T, 1, 1>(p, aligned, stream);
-    if (p.T <= 32) return p.n >= 32 * 128 ? go_few<T, 2, 2>(p, aligned, stream) : go_few<T, 2, 1>(p, aligned, stream);
-    if (p.T <= 64 || row_tiles * ((p.n + 127) / 128) < 256) {
-        if (row_tiles * ((p.n + 63) / 64) >= 128) return go_few<T, 4, 4>(p, aligned, stream);
-        return row_tiles * ((p.n + 31) / 32) >= 128 ? go_few<T, 4, 2>(p, aligned, stream) : go_few<T, 4, 1>(p, aligned, stream);
+    const forms::Project form = forms::project_form(p.T, p.d, p.n, sizeof(T), aligned);
+    if (form.kind == forms::Project::TILES) return go<T, S>(p, stream);
+    if (form.kind == forms::Project::TALL) {
+        switch (form.fm) {
+            case 2: return go_cut<T, 2>(p, sums, form.splits, stream);
+            case 3: return go_cut<T, 3>(p, sums, form.splits, stream);
+            case 4: return go_cut<T, 4>(p, sums, form.splits, stream);
+            case 5: return go_cut<T, 5>(p, sums, form.splits, stream);
+            case 6: return go_cut<T, 6>(p, sums, form.splits, stream);
+            case 7: return go_cut<T, 7>(p, sums, form.splits, stream);
+            default: return go_cut<T, 8>(p, sums, form.splits, stream);
+        }
     }
-    return go<T, S>(p, stream);
+    switch (16 * form.fm + form.fn) {
+        case 16 + 1: return go_few<T, 1, 1>(p, aligned, stream);
+        case 16 + 2: return go_few<T, 1, 2>(p, aligned, stream);
+        case 32 + 1: return go_few<T, 2, 1>(p, aligned, stream);
+        case 32 + 2: return go_few<T, 2, 2>(p, aligned, stream);
+        case 64 + 1: return go_few<T, 4, 1>(p, aligned, stream);
+        case 64 + 2: return go_few<T, 4, 2>(p, aligned, stream);
+        default: return go_few<T, 4, 4>(p, aligned, stream);
+    }
 }
 
 inline int u_stride_bytes(int r, int size) { return (r * size + 15) / 16 * 16; }
