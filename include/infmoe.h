@@ -319,8 +319,8 @@ int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const 
  * ffn_kind: INFMOE_FFN_RELU max(u, 0); _GATED_GELU gelu_tanh(u) * v; _GATED_SILU u / (1 + exp(-u)) * v (wi_1 is NULL with
  * RELU).  x, y [T] rows of d, wi, wi_1 [E] matrices [h][d] that lie wi_stride elements apart, wo [E] matrices [d][h]
  * wo_stride apart (so the experts may be tensors of their own or slots of one packed block), all in `dtype`.  Sums are
- * FP32; the hidden rows are rounded to `dtype` (they are the second product's operand), the weighted sum is FP32, in the
- * order of j, and rounded once.  An id outside [0, E) adds 0 * weights[t][j]: nothing, or NaN where the weight is one.  Ids
+ * FP32; the hidden rows are rounded to `dtype` (they are the second product's operand; in F16 a hidden value beyond 65504
+ * becomes infinite), the weighted sum is FP32, in the order of j, and rounded once.  An id outside [0, E) adds 0 * weights[t][j]: nothing, or NaN where the weight is one.  Ids
  * may repeat.  1 <= E <= 1024, 1 <= k <= 32, T * k <= 2^30, d and h up to 2^23.  A product with more tiles than a launch holds
  * is refused (only from T * k * max(d, h) = 2^36 or, with few rows an expert, E * max(d, h) = 2^27 on).
  * d and h of whole 16-byte pieces and operands on 16-byte boundaries are the fast case, any others are served.  y must not
@@ -338,9 +338,10 @@ int32_t infmoe_experts_topk(int32_t T, int32_t k, int32_t E, int32_t d, int32_t 
  *   y[t] = w x[t] + scale[a] * b_a (a_a x[t]),  a = adapter[t]
  * w [n][d], a [L][r][d], b [L][n][r], x [T] rows of d, y [T] rows of n, all in `dtype`; adapter int32 [T], scale float [L]
  * or NULL (1).  A row whose adapter is outside [0, L) gets w x[t].  Sums are FP32; scale[a] * a_a x[t] is rounded to
- * `dtype` (it is the second product's operand), y once.  What one adapter holds cannot reach the rows of another.
- * 1 <= r <= 256, d and n up to 2^23.  Rows of whole 16-byte pieces on 16-byte boundaries are the fast case.  Rows may come in any order; those
- * of one adapter side by side are the cheap one.  y must not overlap the inputs.
+ * `dtype` (it is the second product's operand; in F16 a value beyond 65504 becomes infinite), y once.  What one adapter holds
+ * cannot reach the rows of another.  1 <= r <= 256, d and n up to 2^23.  Rows of whole 16-byte pieces on 16-byte boundaries
+ * are the fast case.  Rows may come in any order; those of one adapter side by side are the cheap one.  y must not overlap the
+ * inputs.
  * workspace: infmoe_lora_project_workspace_bytes, 256-byte aligned, of any contents, of one call at a time.
  */
 size_t infmoe_lora_project_workspace_bytes(int32_t T, int32_t d, int32_t n, int32_t r, int32_t dtype);

@@ -276,7 +276,9 @@ __global__ __launch_bounds__(kTallThreads) void project_tall_kernel(Args p) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) acc[i][j][q] += mine[i] == a ? sum[q] : 0.f;
                 }
-                __builtin_amdgcn_sched_barrier(0);  // one block's loads at a time: all of them at once do not fit the registers
+                // one block's loads at a time.  (Beside the sums of tall tiles even these do not fit: 8 registers are spilled at 5
+                // blocks, 45 at 6, 82 at 7 and 115 at 8, all of it here and none in the loop over K.)
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll

@@ -120,8 +120,8 @@ def experts_topk(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, wi: 
     """y[t] = sum over j of weights[t, j] * wo[e] act(wi[e] x[t] [, wi_1[e] x[t]]) with e = ids[t, j]: x [T, d], ids int32 and
     weights float32 [T, k] as route_topk gives them, wi, wi_1 [E, h, d], wo [E, d, h] -> [T, d].
 
-    ffn: "relu", "gated_gelu" or "gated_silu" (the gated ones take wi_1).  An id that is no expert adds nothing.  See
-    infmoe_experts_topk."""
+    ffn: "relu", "gated_gelu" or "gated_silu" (the gated ones take wi_1).  An id that is no expert adds nothing.  Hidden rows are
+    held in x's type: in float16 values beyond 65504 become infinite.  See infmoe_experts_topk."""
     _forward_only(x, weights, wi, wo, wi_1, out)
     T, d, x_stride, dtype = _start("x", x)
     device, kind = x.device, capi.TOPK_FFN_KINDS.get(ffn)
