@@ -325,7 +325,8 @@ int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const 
  * is refused (only from T * k * max(d, h) = 2^36 or, with few rows an expert, E * max(d, h) = 2^27 on).
  * d and h of whole 16-byte pieces and operands on 16-byte boundaries are the fast case, any others are served.  y must not
  * overlap the inputs.
- * workspace: infmoe_experts_topk_workspace_bytes, 256-byte aligned, of any contents, of one call at a time.
+ * workspace: infmoe_experts_topk_workspace_bytes (mainly T * k rows of h in `dtype` and of d in FP32), 256-byte aligned, of any
+ * contents, of one call at a time.
  */
 size_t infmoe_experts_topk_workspace_bytes(int32_t T, int32_t k, int32_t E, int32_t d, int32_t h, int32_t dtype);
 int32_t infmoe_experts_topk(int32_t T, int32_t k, int32_t E, int32_t d, int32_t h, int32_t ffn_kind, int32_t dtype, const void* x,

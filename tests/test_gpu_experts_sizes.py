@@ -47,3 +47,30 @@ def test_more_tokens_than_one_launch_has_work_items_for(lib, torch_cuda):
     for part in torch.arange(T, device="cuda").split(1 << 22):
         at = (ids[part, 0].long(), row[part])
         assert ((y[part].double() - want[at]).abs() <= bound[at]).all()
+
+
+def test_many_blocks_in_a_graph_and_on_two_streams(lib, torch_cuda):
+    """The plan of many blocks captured, replayed with other routings and eager work between, and on two streams at once."""
+    torch = torch_cuda
+    from infmoe_amd import ops
+    rng = np.random.default_rng(4)
+    T, k, E = 20011, 2, 100
+    c = draw_experts(torch, rng, T, k, E, 16, 24, "gated_silu", "bfloat16")
+    call = lambda: ops.experts_topk(c["x"], c["ids"], c["weights"], c["wi"], c["wo"], c["wi_1"], ffn="gated_silu")
+    want = call()
+    got, sides = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(3):
+        c["ids"].copy_(torch.from_numpy(rng.integers(-1, E, (T, k)).astype(np.int32)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call())
+        torch.cuda.synchronize()
