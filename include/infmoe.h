@@ -320,9 +320,10 @@ int32_t infmoe_route_topk(int32_t T, int32_t E, int32_t k, int32_t dtype, const 
  * RELU).  x, y [T] rows of d, wi, wi_1 [E] matrices [h][d] that lie wi_stride elements apart, wo [E] matrices [d][h]
  * wo_stride apart (so the experts may be tensors of their own or slots of one packed block), all in `dtype`.  Sums are
  * FP32; the hidden rows are rounded to `dtype` (they are the second product's operand; in F16 a hidden value beyond 65504
- * becomes infinite), the weighted sum is FP32, in the order of j, and rounded once.  An id outside [0, E) adds 0 * weights[t][j]: nothing, or NaN where the weight is one.  Ids
- * may repeat.  1 <= E <= 1024, 1 <= k <= 32, T * k <= 2^30, d and h up to 2^23.  A product with more tiles than a launch holds
- * is refused (only from T * k * max(d, h) = 2^36 or, with few rows an expert, E * max(d, h) = 2^27 on).
+ * becomes infinite), the weighted sum is FP32, in the order of j, and rounded once.  An id outside [0, E) adds
+ * 0 * weights[t][j]: nothing, or NaN where the weight is one.  Ids may repeat.  1 <= E <= 1024, 1 <= k <= 32, T * k <= 2^30,
+ * d and h up to 2^23.  A product with more tiles than a launch holds is refused (only from about T * k * max(d, h, 32) = 2^35 or
+ * E * max(d, h) = 2^27 on).
  * d and h of whole 16-byte pieces and operands on 16-byte boundaries are the fast case, any others are served.  y must not
  * overlap the inputs.
  * workspace: infmoe_experts_topk_workspace_bytes (mainly T * k rows of h in `dtype` and of d in FP32), 256-byte aligned, of any
