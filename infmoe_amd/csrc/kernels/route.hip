@@ -14,7 +14,7 @@
 // over hold minus infinity).  Consecutive experts sit in ascending lanes and slots, so "the lowest index" is "the first
 // lane, then the first slot", and all exchanges are between registers of one wave: no barrier.
 //
-// Bound by vector instructions (131071 rows of 256 experts are 134 MB, 27 us of memory time): a round of the selection is a
+// Bound by vector instructions (131071 rows of 256 experts are 134 MB and 8 MB of results, 23 us at 6.2 TB/s, and take 68): a round of the selection is a
 // maximum over the row and the removal of its place.  With a row per wave that place is scalar arithmetic on the masks of
 // V comparisons; with rows of 16 lanes the same instructions serve four rows.
 #include <hip/hip_bf16.h>
